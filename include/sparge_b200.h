@@ -30,10 +30,12 @@ enum {
   SPARGE_ERR_TOO_LARGE = 4,   /* a size exceeds what the kernel supports: maps to ValueError       */
   SPARGE_ERR_UNSUPPORTED = 5  /* valid request that this build does not implement                  */
 };
-enum { SPARGE_F16 = 0, SPARGE_BF16 = 1 };
+enum { SPARGE_F16 = 0, SPARGE_BF16 = 1, SPARGE_F32 = 2 /* sparge_rotary only */ };
 
 /* Device-side status word values written by sparge_attn_fwd when a bounded wait expires. */
-enum { SPARGE_DEV_OK = 0, SPARGE_DEV_TIMEOUT_PRODUCER = 1, SPARGE_DEV_TIMEOUT_MMA = 2, SPARGE_DEV_TIMEOUT_SOFTMAX = 3 };
+enum { SPARGE_DEV_OK = 0, SPARGE_DEV_TIMEOUT_PRODUCER = 1, SPARGE_DEV_TIMEOUT_MMA = 2, SPARGE_DEV_TIMEOUT_SOFTMAX = 3,
+       SPARGE_DEV_BAD_PAGE = 4,   /* a page or sequence number, or a length, that the cache does not have */
+       SPARGE_DEV_PAGE_HAZARD = 5 /* sparge_copy_pages: a destination named twice, or that is a source too */ };
 
 const char* sparge_strerror(int status);
 int sparge_abi_version(void);
@@ -261,6 +263,126 @@ int sparge_peer_close(void* ptr);
 int sparge_copy_async(void* dst, const void* src, size_t bytes, sparge_stream_t stream);
 int sparge_copy2d_async(void* dst, size_t dpitch, const void* src, size_t spitch, size_t width, size_t height,
                         sparge_stream_t stream);
+
+/* ---------------------------------------------------------------- rotary positions and the paged key/value cache
+ * The reference has no counterpart: its operators begin after the positions and know no cache.
+ *
+ * sparge_rotary turns pairs of channels of q and k [B,H,N,D] by position * frequency:
+ *   (a, b) -> magnitude * (a cos t - b sin t, a sin t + b cos t), t = position * frequencies[pair]
+ * Pairs are (2 i, 2 i + 1) when `interleaved`, else (i, i + pairs), inside the first 2 * pairs channels; the others are
+ * copied. `inverse` turns back (t -> -t): the gradient. With axes > 1 pair i takes the position of the axis whose section
+ * holds it (sections[0] pairs of axis 0, then sections[1] of axis 1 ...). t is formed in 64 bits and reduced to one turn, so
+ * that far positions keep their angles; the products are 32-bit, rounded once.
+ * Strides in elements as {batch, head, token}, last dimension contiguous; positions strides {axis, batch, token}. */
+typedef struct {
+  const void *q, *k;   /* k may be NULL (with k_heads 0) */
+  void *q_out, *k_out;
+  long long q_st[3], k_st[3], q_out_st[3], k_out_st[3];
+  int B, N, q_heads, k_heads, D, dtype;
+  const void* positions; /* int32, or int64 with positions_64 */
+  int positions_64;
+  long long positions_st[3];
+  const double* frequencies; /* [pairs], radians per position */
+  int pairs, axes, sections[4], interleaved, inverse;
+  float magnitude;
+} sparge_rotary_args;
+int sparge_rotary(const sparge_rotary_args* args, sparge_stream_t stream);
+
+/* Where the cache of one layer lies: pages of page_size tokens, k_pages and v_pages [num_pages, kv_heads, page_size, D] with
+ * strides in elements as {page, head, row}, last dimension contiguous, page_size a power of two from 16 to 256.
+ * page_table [sequences, table_width] (rows table_stride apart): the pages of each sequence in order; seq_lens [sequences]:
+ * tokens held, the new ones included. cu_seqlens [sequences + 1]: rows of the packed tokens, sequence i has
+ * cu_seqlens[i] to cu_seqlens[i + 1], its last tokens; NULL: one token each (tokens == sequences). */
+typedef struct {
+  void *k_pages, *v_pages;
+  long long k_st[3], v_st[3];
+  const int32_t *page_table, *seq_lens, *cu_seqlens;
+  long long table_stride;
+  int sequences, table_width, num_pages, page_size, kv_heads, D, dtype, tokens;
+} sparge_cache;
+
+/* Writes the new tokens' k and v [tokens, kv_heads, D] to their pages. With frequencies k is rotated by its position in the
+ * sequence on the way (pairs, interleaved, magnitude as in sparge_rotary), and q [tokens, q_heads, D], if given, to q_out.
+ * Strides {token, head}. Rows of no sequence are not written to pages and give zeros in q_out. A token whose position
+ * has no page (table entry outside the pool, position below 0 or outside the table) is left out of the pages and reported as
+ * SPARGE_DEV_BAD_PAGE. Two tokens never share a place unless two sequences
+ * share the page that they write to, which is the caller's mistake. */
+typedef struct {
+  sparge_cache cache;
+  const void *k, *v, *q;
+  void* q_out;
+  long long k_st[2], v_st[2], q_st[2], q_out_st[2];
+  int q_heads;
+  const double* frequencies;
+  int pairs, interleaved;
+  float magnitude;
+  int32_t* dev_status;
+} sparge_append_args;
+int sparge_append_kv(const sparge_append_args* args, sparge_stream_t stream);
+
+/* Attention of the new tokens over everything their sequences hold in the cache, themselves included.
+ *   out[t, h] = sum over keys k of softmax_k(scale q[t, h] . K[k]) V[k],  lse[t, h] = log sum over k of exp(scale q . K[k])
+ * Query head h reads key head h / (q_heads / kv_heads). is_causal: token j of a sequence's n new ones sees the keys up to its
+ * own position, seq_lens - n + j; else all of the sequence's. A row that sees no key gives zeros and an lse of -inf.
+ * q, out [tokens, q_heads, D] with strides {token, head}, 16-byte aligned rows; D 64 or 128; lse [tokens, q_heads]
+ * contiguous, or NULL. max_chunk: an upper bound of the new tokens of one sequence; it chooses the kernel, results hold
+ * whatever it says. Rows of no sequence: zeros (lse -inf) with zero_rest, else left as they were. Scores, sums and products are
+ * accumulated in 32 bits; probabilities are rounded to the 16-bit type before the product with V. Keys at or behind the
+ * length are never read into a result, whatever their pages hold. A page number outside the pool, or a length outside the
+ * table, is reported as SPARGE_DEV_BAD_PAGE and the rows of that sequence are undefined.
+ * workspace: sparge_paged_attention_workspace_bytes() bytes of device memory, 16-byte aligned, of this call alone. */
+typedef struct {
+  sparge_cache cache;
+  const void* q;
+  void* out;
+  float* lse;
+  long long q_st[2], out_st[2];
+  int q_heads, is_causal, max_chunk, zero_rest;
+  float scale;
+  void* workspace;
+  size_t workspace_bytes;
+  int32_t* dev_status;
+} sparge_paged_attention_args;
+size_t sparge_paged_attention_workspace_bytes(int q_heads, int kv_heads, int D, int max_chunk);
+int sparge_paged_attention(const sparge_paged_attention_args* args, sparge_stream_t stream);
+
+/* Bookkeeping of the pages, all of it on the device: page_table [sequences, table_width] int32 (-1: no page; rows
+ * table_stride apart), seq_lens [sequences], ref_counts [num_pages] (0: free). Free pages are taken lowest first, for one
+ * sequence after the other, so that results do not depend on the order in which threads run. Numbers of sequences outside the
+ * table are reported as SPARGE_DEV_BAD_PAGE and skipped; -1 is skipped silently. workspace: device memory of
+ * sparge_pages_workspace_bytes(sequences or pairs, table_width, num_pages) bytes, contents need no initialisation.
+ *
+ * sparge_allocate_pages: room for new_tokens [sequences] more tokens each; seq_lens grow by them. served [sequences] (0 / 1):
+ * a sequence that the pool or its row of the table has no room for (or new_tokens below 0) keeps its length and gets nothing.
+ * The pool serves the sequences in order: behind the first one that it cannot serve, only those that need no page are.
+ * sparge_free_sequences: releases the pages of `n` sequences and empties their rows. The same sequence twice is released once.
+ * sparge_fork_sequences: sequence dst[i] becomes a copy of src[i] for all i at once (every source is read before any
+ * destination changes). Full pages are shared; a last page that is not full is copied to a fresh page. What the
+ * destinations held before is released, after the fresh pages were taken. served [n]: 0 where there was no page left, or
+ * where a later pair has the same destination; such a destination stays as it was. src[i] == dst[i] does nothing.
+ * sparge_compact_pages: live pages with numbers from the count of live pages up move into the free ones below it, in ascending
+ * order both; table and counts follow. live [1]: the count. Table entries from num_pages up are left as they are.
+ * sparge_copy_pages: page dst[i] becomes a copy of page src[i]. Numbers outside the pool are reported and skipped (-1 silently);
+ * a pair whose destination is another pair's destination or source is reported as SPARGE_DEV_PAGE_HAZARD and not copied.
+ *
+ * pages: `outer` times [num_pages] blocks of page_bytes (a multiple of 16) each: block p of slice o at
+ * o * outer_bytes + p * page_stride_bytes. */
+size_t sparge_pages_workspace_bytes(int n, int table_width, int num_pages);
+int sparge_allocate_pages(int32_t* page_table, int32_t* seq_lens, int32_t* ref_counts, const int32_t* new_tokens,
+                          unsigned char* served, void* workspace, int sequences, int table_width, long long table_stride,
+                          int num_pages, int page_size, sparge_stream_t stream);
+int sparge_free_sequences(int32_t* page_table, int32_t* seq_lens, int32_t* ref_counts, const int32_t* which, int n,
+                          int sequences, int table_width, long long table_stride, int num_pages, int32_t* dev_status,
+                          sparge_stream_t stream);
+int sparge_fork_sequences(void* pages, long long outer, long long outer_bytes, long long page_stride_bytes, long long page_bytes,
+                          int32_t* page_table, int32_t* seq_lens, int32_t* ref_counts, const int32_t* src, const int32_t* dst,
+                          unsigned char* served, void* workspace, int n, int sequences, int table_width,
+                          long long table_stride, int num_pages, int page_size, int32_t* dev_status, sparge_stream_t stream);
+int sparge_compact_pages(void* pages, long long outer, long long outer_bytes, long long page_stride_bytes, long long page_bytes,
+                         int32_t* page_table, int32_t* ref_counts, int32_t* live, void* workspace, int sequences,
+                         int table_width, long long table_stride, int num_pages, sparge_stream_t stream);
+int sparge_copy_pages(void* pages, long long outer, long long outer_bytes, long long page_stride_bytes, long long page_bytes,
+                      const int32_t* src, const int32_t* dst, int n, int num_pages, int32_t* dev_status, sparge_stream_t stream);
 
 #ifdef __cplusplus
 }

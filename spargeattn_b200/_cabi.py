@@ -56,6 +56,17 @@ SIGNATURES = {
     "sparge_attn_fwd": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _f, _p]),
     "sparge_div_approx": (_i, [_p, _p, _p, _i, _p]),
     "sparge_tensor_peak": (_i, [_i, _i, _i, _i, _p, ctypes.POINTER(ctypes.c_float), ctypes.POINTER(ctypes.c_double), _p]),
+    # the argument structures are laid out by the header; Python reaches these entries through the native binding
+    "sparge_rotary": (_i, [_p, _p]),
+    "sparge_append_kv": (_i, [_p, _p]),
+    "sparge_paged_attention_workspace_bytes": (_sz, [_i, _i, _i, _i]),
+    "sparge_paged_attention": (_i, [_p, _p]),
+    "sparge_pages_workspace_bytes": (_sz, [_i, _i, _i]),
+    "sparge_allocate_pages": (_i, [_p, _p, _p, _p, _p, _p, _i, _i, _ll, _i, _i, _p]),
+    "sparge_free_sequences": (_i, [_p, _p, _p, _p, _i, _i, _i, _ll, _i, _p, _p]),
+    "sparge_fork_sequences": (_i, [_p, _ll, _ll, _ll, _ll, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _ll, _i, _i, _p, _p]),
+    "sparge_compact_pages": (_i, [_p, _ll, _ll, _ll, _ll, _p, _p, _p, _p, _i, _i, _ll, _i, _p]),
+    "sparge_copy_pages": (_i, [_p, _ll, _ll, _ll, _ll, _p, _p, _i, _i, _p, _p]),
 }
 for _name, (_res, _args) in SIGNATURES.items():
     _fn = getattr(lib, _name)

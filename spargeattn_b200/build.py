@@ -13,7 +13,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libsparge_b200.so")
 BINDING = os.path.join(HERE, "_binding.so")
 SOURCES = ["cabi.cu", "kmean.cu", "pool_quant.cu", "prep.cu", "select.cu", "quant_v.cu", "attn_sm100.cu", "peer.cu", "tensor_peak.cu",
-           "forward.cu"]
+           "forward.cu", "rotary.cu", "pages.cu", "paged_decode.cu", "paged_attention.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",
               "-Xptxas", "-v"]
 
@@ -31,8 +31,8 @@ def _stale(target, deps):
 
 
 def _build_binding(headers, force):
-    src = os.path.join(CSRC, "binding.cpp")
-    if not (force or _stale(BINDING, [src] + headers)):
+    sources = [os.path.join(CSRC, f) for f in ("binding.cpp", "cache_binding.cpp")]
+    if not (force or _stale(BINDING, sources + headers)):
         return
     import sysconfig
     import torch
@@ -40,15 +40,15 @@ def _build_binding(headers, force):
     cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
     cmd += [f"-isystem{p}" for p in include_paths() + [sysconfig.get_paths()["include"], os.path.join(cuda, "include")]]
-    cmd += [src, "-o", BINDING, LIB, "-Wl,-rpath,$ORIGIN"] + [f"-L{p}" for p in library_paths()]
+    cmd += sources + ["-o", BINDING, LIB, "-Wl,-rpath,$ORIGIN"] + [f"-L{p}" for p in library_paths()]
     cmd += ["-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError(f"g++ failed for binding.cpp:\n{r.stdout}\n{r.stderr}")
+        raise RuntimeError(f"g++ failed for the binding:\n{r.stdout}\n{r.stderr}")
 
 
 def build(force=False, verbose=False):
-    headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".cuh")]
+    headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))]
     headers.append(os.path.join(HERE, "..", "include", "sparge_b200.h"))
     objdir = os.path.join(HERE, "build")
     os.makedirs(objdir, exist_ok=True)

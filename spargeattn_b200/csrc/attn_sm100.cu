@@ -33,6 +33,7 @@
 #include "row_groups.cuh"
 #include "sm100_ptx.cuh"
 #include "step_word.cuh"
+#include "tensor_map.cuh"
 
 namespace sparge {
 
@@ -703,23 +704,9 @@ attn_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ 
 }
 
 // ---------------------------------------------------------------------------- host side
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = []() -> EncodeTiledFn {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess) return nullptr;
-    return reinterpret_cast<EncodeTiledFn>(p);
-  }();
-  return fn;
-}
-
 // Byte tensor [planes, rows, inner] with a [1, box_rows, inner] box, swizzle span = inner bytes.
 static bool make_map(CUtensorMap* m, const void* ptr, uint64_t inner, uint64_t rows, uint64_t planes, uint32_t box_rows) {
-  EncodeTiledFn enc = encode_fn();
+  EncodeTiledFn enc = encode_tiled();
   if (!enc) return false;
   cuuint64_t dims[3] = {inner, rows, planes};
   cuuint64_t strides[2] = {inner, inner * rows};
@@ -734,7 +721,7 @@ static bool make_map(CUtensorMap* m, const void* ptr, uint64_t inner, uint64_t r
 // fp16 V as bytes, any strides: [B, H, N, 2 D], copied as 64 rows of 128 bytes (64 channels; x is 0 or 128); rows past N
 // read as zeros.
 static bool make_map_v16(CUtensorMap* m, const AttnArgs& a) {
-  EncodeTiledFn enc = encode_fn();
+  EncodeTiledFn enc = encode_tiled();
   if (!enc) return false;
   cuuint64_t dims[4] = {2 * (cuuint64_t)a.D, (cuuint64_t)a.N, (cuuint64_t)a.H, (cuuint64_t)a.B};
   cuuint64_t strides[3] = {2 * (cuuint64_t)a.v_st[2], 2 * (cuuint64_t)a.v_st[1], 2 * (cuuint64_t)a.v_st[0]};
@@ -745,19 +732,6 @@ static bool make_map_v16(CUtensorMap* m, const AttnArgs& a) {
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Function attributes are per device and outlive the call: set once for each (kernel, device).
-static bool attn_attributes(const void* kern, int smem, std::atomic<uint64_t>& done) {
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return false;
-  const uint64_t bit = 1ull << (dev & 63);
-  if (dev < 64 && (done.load(std::memory_order_acquire) & bit)) return true;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return false;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) != cudaSuccess)
-    return false;
-  if (dev < 64) done.fetch_or(bit, std::memory_order_release);
-  return true;
-}
-
 template <int D, bool CAUSAL, int PV_MODE, typename OutT, int GRAN, bool PVF16, bool ORDERED = false>
 static int launch_attn(const AttnArgs& a, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t st) {
   if (GRAN == 1 && PV_MODE != 2 && !ORDERED && !a.q_ranges && !a.pv_count && (a.row_order || (a.order_groups > 0 && a.order_groups < a.B * a.H)))
@@ -765,7 +739,7 @@ static int launch_attn(const AttnArgs& a, const CUtensorMap& tq, const CUtensorM
   auto kern = attn_kernel<D, CAUSAL, PV_MODE, OutT, GRAN, PVF16, ORDERED>;
   constexpr int smem = AttnShape<D, PVF16>::kSmemBytes;
   static std::atomic<uint64_t> done{0};
-  if (!attn_attributes((const void*)kern, smem, done)) return SPARGE_ERR_CUDA;
+  if (!kernel_attributes((const void*)kern, smem, done)) return SPARGE_ERR_CUDA;
   const int nq = (a.N + 127) / 128, nk = (a.N + 63) / 64;
   const int gx = a.q_ranges ? min(a.q_blocks_max, nq) : nq;
   const cudaError_t e = launch(kern, dim3(gx, a.B * a.H), kAttnThreads, smem, st, a.dependent, tq, tk, tv, (OutT*)a.o, a.lut,

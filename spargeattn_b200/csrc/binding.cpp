@@ -24,6 +24,7 @@
 #include <mutex>
 #include <tuple>
 
+#include "cache_binding.h"
 #include "forward.cuh"
 
 namespace {
@@ -219,4 +220,10 @@ PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, kMethods,
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__binding() { return PyModule_Create(&kModule); }
+at::Tensor* cache_status_word(int device) { return device >= 0 && device < 64 ? status_words[device] : nullptr; }
+
+PyMODINIT_FUNC PyInit__binding() {
+  PyObject* m = PyModule_Create(&kModule);
+  if (m && PyModule_AddFunctions(m, kCacheMethods) < 0) Py_CLEAR(m);
+  return m;
+}

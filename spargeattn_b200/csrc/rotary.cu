@@ -1,0 +1,349 @@
+// Rotary positions, and the write of new tokens into a paged key/value cache, which turns keys and queries on its way.
+//
+//   (a, b) -> magnitude (a cos t - b sin t, a sin t + b cos t),  t = position * frequency
+//
+// The phase is formed in 64 bits and reduced to half a turn before it becomes a float: at position 10^6 a phase of 32 bits is
+// off by 0.06 radians. The products are 32-bit and rounded once to the tensor's type.
+//
+// Every element is read and written once, so HBM bounds it; what the kernel must not do is spend its time on the angles. A
+// phase and its sine cost about 60 instructions, and a token's pairs are the same for all its heads: a block computes those of
+// its tokens once into shared memory, and a thread keeps the ones of its channels in registers while it walks the heads.
+#include "common.cuh"
+
+namespace sparge {
+
+constexpr int kRotThreads = 256;
+constexpr int kRotTokens = 8;      // most tokens of a block
+
+struct RotSlot {                   // q, k or v
+  const void* x;
+  void* y;                         // paged: the pages
+  long long xb, xh, xn;            // strides of the source: batch, head, token
+  long long yb, yh, yn;            // of the destination; paged: page, head, row
+  int heads;
+  bool rotate, paged;
+};
+
+struct RotParams {
+  RotSlot slot[3];
+  int slots, B, N, D, pairs, axes, sections[4];
+  const void* positions;
+  bool pos64, inverse;
+  long long pos_st[3];
+  const double* freq;
+  float magnitude;
+  int tokens_per_block;
+  // append
+  const int32_t *table, *seq_lens, *cu;
+  long long table_stride;
+  int sequences, width, num_pages, page_size;
+  int32_t* dev_status;
+};
+
+// V consecutive elements as they lie in memory.
+template <typename T, int V>
+struct Raw {
+  T v[V];
+};
+template <typename T, int V, bool VEC>
+__device__ __forceinline__ Raw<T, V> raw_load(const T* p) {
+  Raw<T, V> r;
+  if constexpr (VEC) {
+    constexpr int kWords = V * (int)sizeof(T) / 16;
+    uint4 w[kWords];
+#pragma unroll
+    for (int i = 0; i < kWords; i++) w[i] = reinterpret_cast<const uint4*>(p)[i];
+    memcpy(&r, w, sizeof(r));
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i++) r.v[i] = p[i];
+  }
+  return r;
+}
+template <typename T, int V, bool VEC>
+__device__ __forceinline__ void raw_store(T* p, const Raw<T, V>& r) {
+  if constexpr (VEC) {
+    constexpr int kWords = V * (int)sizeof(T) / 16;
+    uint4 w[kWords];
+    memcpy(w, &r, sizeof(r));
+#pragma unroll
+    for (int i = 0; i < kWords; i++) reinterpret_cast<uint4*>(p)[i] = w[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i++) p[i] = r.v[i];
+  }
+}
+
+template <>
+struct Elem<float> {
+  static __device__ __forceinline__ float to_float(float v) { return v; }
+  static __device__ __forceinline__ float from_float(float v) { return v; }
+};
+
+// The heads of one slot for one token: the thread's unit of channels, heads h0, h0 + step, ... Four heads are loaded before the
+// first is turned: with one at a time the loads of a thread waited for one another.
+template <typename T, int V, bool VEC, bool INTER>
+__device__ __forceinline__ void turn_heads(const T* x, T* y, long long xh, long long yh, int heads, int h0, int step, int unit,
+                                           int rot_units, int pairs, const float2* cs, bool zero) {
+  constexpr int P = INTER ? V / 2 : V;   // pairs of a unit
+  constexpr int kAhead = 4;
+  if (unit < rot_units) {
+    float2 c[P];
+#pragma unroll
+    for (int i = 0; i < P; i++) c[i] = cs[unit * P + i];
+    const int at = unit * V;
+    for (int h = h0; h < heads; h += kAhead * step) {
+      Raw<T, V> a[kAhead], b[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; j++) {
+        const int hj = h + j * step;
+        if (hj < heads && !zero) {
+          a[j] = raw_load<T, V, VEC>(x + hj * xh + at);
+          if (!INTER) b[j] = raw_load<T, V, VEC>(x + hj * xh + pairs + at);
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; i++) a[j].v[i] = b[j].v[i] = Elem<T>::from_float(0.f);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; j++) {
+        const int hj = h + j * step;
+        if (hj >= heads) break;
+        if (INTER) {
+#pragma unroll
+          for (int i = 0; i < P; i++) {
+            const float u = Elem<T>::to_float(a[j].v[2 * i]), w = Elem<T>::to_float(a[j].v[2 * i + 1]);
+            a[j].v[2 * i] = Elem<T>::from_float(u * c[i].x - w * c[i].y);
+            a[j].v[2 * i + 1] = Elem<T>::from_float(u * c[i].y + w * c[i].x);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < P; i++) {
+            const float u = Elem<T>::to_float(a[j].v[i]), w = Elem<T>::to_float(b[j].v[i]);
+            a[j].v[i] = Elem<T>::from_float(u * c[i].x - w * c[i].y);
+            b[j].v[i] = Elem<T>::from_float(u * c[i].y + w * c[i].x);
+          }
+          raw_store<T, V, VEC>(y + hj * yh + pairs + at, b[j]);
+        }
+        raw_store<T, V, VEC>(y + hj * yh + at, a[j]);
+      }
+    }
+  } else {   // channels behind the rotated ones
+    const int at = 2 * pairs + (unit - rot_units) * V;
+    for (int h = h0; h < heads; h += kAhead * step) {
+      Raw<T, V> a[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; j++) {
+        const int hj = h + j * step;
+        if (hj < heads && !zero) a[j] = raw_load<T, V, VEC>(x + hj * xh + at);
+        else {
+#pragma unroll
+          for (int i = 0; i < V; i++) a[j].v[i] = Elem<T>::from_float(0.f);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; j++) {
+        const int hj = h + j * step;
+        if (hj < heads) raw_store<T, V, VEC>(y + hj * yh + at, a[j]);
+      }
+    }
+  }
+}
+
+// V elements make a unit of the copied channels and half a unit of (i, i + pairs); VEC: 16-byte accesses.
+template <typename T, int V, bool VEC, bool INTER, bool PAGED>
+__global__ void __launch_bounds__(kRotThreads) rotary_kernel(const __grid_constant__ RotParams p) {
+  extern __shared__ float2 s_cs[];                  // [tokens_per_block][pairs]
+  __shared__ int s_page[kRotTokens], s_row[kRotTokens], s_pos[kRotTokens];   // paged: -1 no page; row -1 behind the last sequence
+  __shared__ int s_seq;
+  const int tid = threadIdx.x, TOK = p.tokens_per_block;
+  const long long tokens = (long long)p.B * p.N, t0 = (long long)blockIdx.x * TOK;
+
+  if (PAGED) {
+    // the sequence of the block's first token: how many of them end at or before it
+    int seq = 0;
+    if (p.cu) {
+      if (tid == 0) s_seq = 0;
+      __syncthreads();
+      int ended = 0;
+      for (int i = tid; i < p.sequences; i += kRotThreads) ended += p.cu[i + 1] <= t0;
+      if (ended) atomicAdd(&s_seq, ended);
+      __syncthreads();
+      seq = s_seq;
+    }
+    if (tid < TOK) {
+      const long long t = t0 + tid;
+      int page = -1, row = -1, pos = 0;
+      if (t < tokens) {
+        long long end = t + 1;
+        if (p.cu) {
+          while (seq < p.sequences && p.cu[seq + 1] <= t) seq++;
+          if (seq < p.sequences && t < p.cu[seq]) seq = p.sequences;   // in front of the first
+          if (seq < p.sequences) end = p.cu[seq + 1];
+        } else {
+          seq = (int)t;
+        }
+        if (seq < p.sequences) {
+          const long long at = (long long)p.seq_lens[seq] - (end - t);
+          row = 0;
+          if (at >= 0 && at < (long long)p.width * p.page_size) {
+            pos = (int)at;
+            row = pos & (p.page_size - 1);
+            page = p.table[seq * p.table_stride + pos / p.page_size];
+            if (page < 0 || page >= p.num_pages) page = -1;
+          }
+          if (page < 0 && p.dev_status) atomicCAS(p.dev_status, 0, SPARGE_DEV_BAD_PAGE);
+        }
+      }
+      s_page[tid] = page, s_row[tid] = row, s_pos[tid] = pos;
+    }
+    __syncthreads();
+  }
+
+  for (int i = tid; i < TOK * p.pairs; i += kRotThreads) {
+    const int tok = i / p.pairs, pair = i - tok * p.pairs;
+    const long long t = t0 + tok;
+    if (t >= tokens) break;
+    double pos;
+    if (PAGED) {
+      pos = s_pos[tok];
+    } else {
+      int axis = 0;
+      for (int first = 0; axis + 1 < p.axes && pair >= first + p.sections[axis]; axis++) first += p.sections[axis];
+      const int b = (int)(t / p.N);
+      const long long at = axis * p.pos_st[0] + b * p.pos_st[1] + (t - (long long)b * p.N) * p.pos_st[2];
+      pos = p.pos64 ? (double)reinterpret_cast<const long long*>(p.positions)[at]
+                    : (double)reinterpret_cast<const int32_t*>(p.positions)[at];
+    }
+    double turn = pos * p.freq[pair] * 0.15915494309189533577;   // in turns
+    turn -= rint(turn);
+    float s, c;
+    sincospif((float)(2.0 * turn), &s, &c);
+    s_cs[i] = make_float2(c * p.magnitude, (p.inverse ? -s : s) * p.magnitude);
+  }
+  __syncthreads();
+
+  for (int j = 0; j < p.slots; j++) {
+    const RotSlot& sl = p.slot[j];
+    const int pairs = sl.rotate ? p.pairs : 0;
+    const int rot_units = INTER ? 2 * pairs / V : pairs / V;
+    const int units = rot_units + (p.D - 2 * pairs) / V;
+    const int per = min(units, kRotThreads);           // threads of one token's head
+    const int groups = kRotThreads / per, group = tid / per;
+    const int step = max(1, groups / TOK);             // heads side by side
+    for (int g = group; g < TOK * step && group < groups; g += groups) {
+      const int tok = g % TOK, h0 = g / TOK;
+      const long long t = t0 + tok;
+      if (t >= tokens) continue;
+      const int b = PAGED ? 0 : (int)(t / p.N);
+      const T* x = reinterpret_cast<const T*>(sl.x) + b * sl.xb + (t - (long long)b * p.N) * sl.xn;
+      T* y = reinterpret_cast<T*>(sl.y);
+      bool zero = false;
+      if (PAGED && sl.paged) {
+        if (s_page[tok] < 0) continue;
+        y += s_page[tok] * sl.yb + s_row[tok] * sl.yn;
+      } else {
+        zero = PAGED && s_row[tok] < 0;
+        y += b * sl.yb + (t - (long long)b * p.N) * sl.yn;
+      }
+      for (int u = tid - group * per; u < units; u += per)
+        turn_heads<T, V, VEC, INTER>(x, y, sl.xh, sl.yh, sl.heads, h0, step, u, rot_units, pairs, s_cs + tok * p.pairs, zero);
+    }
+  }
+}
+
+template <typename T, bool INTER, bool PAGED>
+static int rotary_launch(RotParams& p, bool vec, cudaStream_t st) {
+  const long long tokens = (long long)p.B * p.N;
+  // Few tokens: a block each, so that a step's heads spread over the GPU; many: eight, whose angles share one pass.
+  p.tokens_per_block = tokens >= 8 * 148 ? kRotTokens : tokens >= 2 * 148 ? 2 : 1;
+  const size_t smem = sizeof(float2) * p.tokens_per_block * p.pairs;
+  const long long blocks = (tokens + p.tokens_per_block - 1) / p.tokens_per_block;
+  if (blocks > 0x7fffffffLL) return SPARGE_ERR_TOO_LARGE;
+  if (vec) rotary_kernel<T, 8, true, INTER, PAGED><<<(unsigned)blocks, kRotThreads, smem, st>>>(p);
+  else rotary_kernel<T, INTER ? 2 : 1, false, INTER, PAGED><<<(unsigned)blocks, kRotThreads, smem, st>>>(p);
+  return launch_status();
+}
+
+// 16-byte accesses of 8 elements: the base, every stride and the channels' borders have to be multiples of them.
+static bool vec_ok(const RotParams& p, bool inter, int elem) {
+  if (p.D % 8 || (p.pairs && (inter ? p.pairs % 4 : p.pairs % 8))) return false;
+  for (int j = 0; j < p.slots; j++) {
+    const RotSlot& s = p.slot[j];
+    if (reinterpret_cast<uintptr_t>(s.x) % 16 || reinterpret_cast<uintptr_t>(s.y) % 16) return false;
+    for (long long st : {s.xb, s.xh, s.xn, s.yb, s.yh, s.yn})
+      if (st * elem % 16) return false;
+  }
+  return true;
+}
+
+template <bool PAGED>
+static int rotary_dispatch(RotParams& p, bool inter, int dtype, cudaStream_t st) {
+  const bool vec = vec_ok(p, inter, dtype == SPARGE_F32 ? 4 : 2);
+#define SPARGE_ROT(T) (inter ? rotary_launch<T, true, PAGED>(p, vec, st) : rotary_launch<T, false, PAGED>(p, vec, st))
+  if (dtype == SPARGE_BF16) return SPARGE_ROT(__nv_bfloat16);
+  if (dtype == SPARGE_F16) return SPARGE_ROT(__half);
+  if constexpr (!PAGED) return SPARGE_ROT(float);
+  return SPARGE_ERR_INVALID_ARG;
+#undef SPARGE_ROT
+}
+
+static RotSlot rot_slot(const void* x, void* y, const long long* xs, const long long* ys, int heads) {
+  return RotSlot{x, y, xs[0], xs[1], xs[2], ys[0], ys[1], ys[2], heads, true, false};
+}
+
+}  // namespace sparge
+
+extern "C" int sparge_rotary(const sparge_rotary_args* a, sparge_stream_t stream) {
+  using namespace sparge;
+  if (!a) return SPARGE_ERR_NULL;
+  if (a->B < 0 || a->N < 0 || a->q_heads < 0 || a->k_heads < 0 || a->D <= 0 || a->D % 2 || a->D > 1024 || a->pairs <= 0 || 2 * a->pairs > a->D ||
+      a->dtype < 0 || a->dtype > SPARGE_F32 || a->axes < 1 || a->axes > 4)
+    return SPARGE_ERR_INVALID_ARG;
+  if (a->axes > 1) {
+    int sum = 0;
+    for (int i = 0; i < a->axes; i++) {
+      if (a->sections[i] < 0) return SPARGE_ERR_INVALID_ARG;
+      sum += a->sections[i];
+    }
+    if (sum != a->pairs) return SPARGE_ERR_INVALID_ARG;
+  }
+  if ((long long)a->B * a->N == 0 || a->q_heads + a->k_heads == 0) return SPARGE_OK;
+  if ((a->q_heads && (!a->q || !a->q_out)) || (a->k_heads && (!a->k || !a->k_out)) || !a->positions || !a->frequencies) return SPARGE_ERR_NULL;
+  RotParams p = {};
+  if (a->q_heads) p.slot[p.slots++] = rot_slot(a->q, a->q_out, a->q_st, a->q_out_st, a->q_heads);
+  if (a->k_heads) p.slot[p.slots++] = rot_slot(a->k, a->k_out, a->k_st, a->k_out_st, a->k_heads);
+  p.B = a->B, p.N = a->N, p.D = a->D, p.pairs = a->pairs, p.axes = a->axes;
+  for (int i = 0; i < 4; i++) p.sections[i] = a->sections[i];
+  p.positions = a->positions, p.pos64 = a->positions_64 != 0, p.inverse = a->inverse != 0;
+  for (int i = 0; i < 3; i++) p.pos_st[i] = a->positions_st[i];
+  p.freq = a->frequencies, p.magnitude = a->magnitude;
+  return rotary_dispatch<false>(p, a->interleaved != 0, a->dtype, (cudaStream_t)stream);
+}
+
+extern "C" int sparge_append_kv(const sparge_append_args* a, sparge_stream_t stream) {
+  using namespace sparge;
+  if (!a) return SPARGE_ERR_NULL;
+  const sparge_cache& c = a->cache;
+  if (c.tokens < 0 || c.sequences < 0 || c.kv_heads <= 0 || c.D <= 0 || c.D % 8 || c.D > 1024 || (c.dtype != SPARGE_F16 && c.dtype != SPARGE_BF16) ||
+      c.page_size < 16 || c.page_size > 256 || (c.page_size & (c.page_size - 1)) || c.table_width < 0 || c.num_pages < 0 ||
+      (!c.cu_seqlens && c.tokens != c.sequences) || (a->q && a->q_heads <= 0))
+    return SPARGE_ERR_INVALID_ARG;
+  if (a->frequencies && (a->pairs <= 0 || 2 * a->pairs > c.D)) return SPARGE_ERR_INVALID_ARG;
+  if (a->q && !a->frequencies) return SPARGE_ERR_INVALID_ARG;
+  if ((long long)c.table_width * c.page_size > 0x7fffffffLL) return SPARGE_ERR_TOO_LARGE;
+  if (c.tokens == 0) return SPARGE_OK;
+  if (!a->k || !a->v || (c.num_pages && (!c.k_pages || !c.v_pages)) || (a->q && !a->q_out)) return SPARGE_ERR_NULL;
+  if (c.sequences && (!c.seq_lens || (c.table_width && !c.page_table))) return SPARGE_ERR_NULL;
+  RotParams p = {};
+  const auto paged = [&](const void* x, const long long* xs, void* pages, const long long* ps, bool rotate) {
+    p.slot[p.slots++] = RotSlot{x, pages, 0, xs[1], xs[0], ps[0], ps[1], ps[2], c.kv_heads, rotate, true};
+  };
+  if (a->q) p.slot[p.slots++] = RotSlot{a->q, a->q_out, 0, a->q_st[1], a->q_st[0], 0, a->q_out_st[1], a->q_out_st[0], a->q_heads, true, false};
+  paged(a->k, a->k_st, c.k_pages, c.k_st, a->frequencies != nullptr);
+  paged(a->v, a->v_st, c.v_pages, c.v_st, false);
+  p.B = 1, p.N = c.tokens, p.D = c.D, p.pairs = a->frequencies ? a->pairs : 0, p.axes = 1, p.freq = a->frequencies, p.magnitude = a->magnitude;
+  p.table = c.page_table, p.seq_lens = c.seq_lens, p.cu = c.cu_seqlens, p.table_stride = c.table_stride;
+  p.sequences = c.sequences, p.width = c.table_width, p.num_pages = c.num_pages, p.page_size = c.page_size, p.dev_status = a->dev_status;
+  return rotary_dispatch<true>(p, a->interleaved != 0, c.dtype, (cudaStream_t)stream);
+}

@@ -84,9 +84,14 @@ def device_status_word(device) -> torch.Tensor:
 
 
 def check_device_status(device=None) -> int:
-    """Synchronising read of the device status word; raises if a kernel reported a timeout."""
+    """Synchronising read of the device status word; raises if a kernel reported a timeout, or a cache that names what it does
+    not have. The word keeps the first report."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     code = int(device_status_word(dev).item())
+    if code == 4:
+        raise RuntimeError("device status 4: a page or sequence number, or a length, that the cache does not have")
+    if code == 5:
+        raise RuntimeError("device status 5: copy_pages was given a destination twice, or one that is a source too")
     if code != 0:
         raise RuntimeError(f"sparge_attn_fwd reported device status {code} (a bounded wait expired)")
     return code
