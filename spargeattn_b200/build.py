@@ -13,7 +13,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libsparge_b200.so")
 BINDING = os.path.join(HERE, "_binding.so")
 SOURCES = ["cabi.cu", "kmean.cu", "pool_quant.cu", "prep.cu", "select.cu", "quant_v.cu", "attn_sm100.cu", "peer.cu", "tensor_peak.cu",
-           "forward.cu", "rotary.cu", "pages.cu", "paged_decode.cu", "paged_attention.cu"]
+           "forward.cu", "rotary.cu", "pages.cu", "paged_decode.cu", "paged_tile.cu", "paged_attention.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",
               "-Xptxas", "-v"]
 

@@ -35,8 +35,8 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedParams p, int rows
   for (int d = 0; d < D / 32; d++) acc[d] = 0.f;
   for (int i0 = 0; i0 < pieces; i0 += 32) {
     float w = 0.f;
-    if (i0 + lane < pieces && top != -INFINITY) {
-      w = ex2_approx(p.part_ml[slot(i0 + lane) * 2] - top);
+    if (i0 + lane < pieces) {
+      w = top == -INFINITY ? 1.f : ex2_approx(p.part_ml[slot(i0 + lane) * 2] - top);   // (no key seen: sums of 0, or of NaN)
       sum += w * p.part_ml[slot(i0 + lane) * 2 + 1];
     }
     const int here = min(32, pieces - i0);
@@ -55,13 +55,13 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedParams p, int rows
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  const float inv = sum != 0.f ? 1.f / sum : 0.f;
   const int seq_row = a.row + r, tok = seq_row / p.group, head = a.head * p.group + seq_row - tok * p.group;
   T* dst = reinterpret_cast<T*>(p.out) + (long long)(a.token + tok) * p.out_token + (long long)head * p.out_head + lane * (D / 32);
 #pragma unroll
   for (int d = 0; d < D / 32; d++) dst[d] = Elem<T>::from_float(acc[d] * inv);
   if (p.lse && lane == 0)
-    p.lse[(long long)(a.token + tok) * (p.kv_heads * p.group) + head] = sum > 0.f ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+    p.lse[(long long)(a.token + tok) * (p.kv_heads * p.group) + head] = sum != 0.f ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
 }
 
 // 16-bit pages [pages, heads, page_size, D] by their strides; a copy takes up to kBlockKeys rows of 64 channels of one page.
@@ -76,10 +76,8 @@ static bool page_map(CUtensorMap* m, const void* ptr, const long long* st, const
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-static int tile_rows(int group, int max_chunk) {
-  (void)group, (void)max_chunk;
-  return kDecodeRows;
-}
+// Which kernel: tiles of 16 rows or of 256.
+static int tile_rows(int group, int max_chunk) { return (long long)group * max_chunk <= kDecodeRows ? kDecodeRows : kTileRows; }
 
 static size_t starts_bytes(int shares) { return (sizeof(ShareStart) * (shares + 1) + 255) / 256 * 256; }
 
@@ -125,7 +123,7 @@ extern "C" int sparge_paged_attention(const sparge_paged_attention_args* a, spar
   p.part_ml = p.part_o + (size_t)p.max_shares * 2 * rows * c.D;
   p.dev_status = a->dev_status;
   const cudaStream_t st = (cudaStream_t)stream;
-  const int rc = paged_decode_launch(p, k, v, c.D, c.dtype, st);
+  const int rc = rows == kDecodeRows ? paged_decode_launch(p, k, v, c.D, c.dtype, st) : paged_tile_launch(p, k, v, c.D, c.dtype, st);
   if (rc != SPARGE_OK || p.max_shares < 2) return rc;
   const dim3 grid(p.max_shares - 1, (rows + 7) / 8);
 #define SPARGE_JOIN(T, D) launch(paged_join_kernel<T, D>, grid, dim3(256), 0, st, true, p, rows)

@@ -300,7 +300,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       if (r < u.rows) {
         if (u.flags & kWhole) {
           const int seq_row = u.row + r, tok = seq_row / p.group, head = u.head * p.group + seq_row - tok * p.group;
-          const float inv = sum > 0.f ? 1.f / sum : 0.f;
+          const float inv = sum != 0.f ? 1.f / sum : 0.f;
           T* dst = reinterpret_cast<T*>(p.out) + (long long)(u.token + tok) * p.out_token + (long long)head * p.out_head + part * C;
 #pragma unroll
           for (int c = 0; c < C; c += 8) {
@@ -310,7 +310,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             *reinterpret_cast<uint4*>(dst + c) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
           }
           if (p.lse && part == 0)
-            p.lse[(long long)(u.token + tok) * (p.kv_heads * p.group) + head] = sum > 0.f ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+            p.lse[(long long)(u.token + tok) * (p.kv_heads * p.group) + head] = sum != 0.f ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
         } else {
           const long long at_row = ((long long)blockIdx.x * 2 + (u.flags & kHead ? 0 : 1)) * R + r;
           float* dst = p.part_o + at_row * D + part * C;

@@ -1,0 +1,422 @@
+// Attention of chunks of new tokens over a paged cache: tiles of 256 rows on the 5th-generation tensor cores.
+//
+//   S = Q K^T   tcgen05.mma kind::f16, Q and K from 128B-swizzled shared memory, 128 rows by 128 keys, f32 in tensor memory
+//   softmax     one thread per row: maximum, exponentials, sum in registers; P rounded to the 16-bit type and stored over S
+//   O += P V    tcgen05.mma kind::f16 with P from tensor memory and V token-major (an MN-major operand), f32 in tensor memory
+//
+// A CTA has two tiles of 128 rows (the rows of one key head: tokens by query heads of its group, so grouped heads share every
+// key that is fetched) and works on both in turn: while the softmax warps of one are busy, the tensor cores do P V and the next
+// Q K^T of the other. Their S, P and O fill tensor memory: columns [0, 128) S and P of the first, [128, 256) of the second,
+// [256, 384) and [384, 512) their outputs. 10 warps: 0-3 and 4-7 softmax and epilogue of a tile each, 8 the copies, 9 the
+// products. One CTA on each SM takes an equal run of the call's units (paged_schedule.cuh); the copies run ahead over the borders
+// of tiles, heads and sequences, and a tile's queries are fetched while the last product of the tile before it is under way.
+//
+// The products of a step of 128 keys take 1 024 cycles for the two tiles at D = 128 and the exponentials as many (16 a cycle on
+// an SM), so both have to run all the time. The running maximum moves only when a row's maximum grows by more than 2^8
+// (probabilities up to 256 round as exactly as ones up to 1), so that the output is hardly ever rescaled.
+//
+// Every wait is bounded; on expiry the kernel reports and unwinds.
+#include <atomic>
+
+#include "launch.cuh"
+#include "paged.cuh"
+
+namespace sparge {
+
+constexpr int kTileThreads = 320, kLoadWarp = 8, kMmaWarpT = 9;
+constexpr int kTileRing = 8;                     // tiles whose description may wait to be read
+constexpr float kRescaleFrom = 8.f;              // in log2
+
+template <int D>
+struct TileShape {
+  static constexpr int kQ = 128 * D * 2;                       // one tile's queries
+  static constexpr int kTile = kBlockKeys * D * 2;             // K or V of a unit
+  static constexpr int kSlots = D == 128 ? 5 : 8;
+  static constexpr int kSmemBytes = 1024 + 2 * kQ + kSlots * kTile;
+};
+
+// What a tile's roles have to know.
+struct TileWork {
+  int units;                      // of this share
+  int key;                        // first key
+  int token, row, rows, head, length, visible0, flags;
+};
+
+// D[tmem] (+)= A[tmem] * B[smem], 16-bit inputs of one type, f32 accumulate, K = 16.
+__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack_probs(float a, float b) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kTileThreads, 1)
+paged_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PagedParams p) {
+  using Shape = TileShape<D>;
+  constexpr int NS = Shape::kSlots;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* s_ring = smem + 2 * Shape::kQ;
+  __shared__ uint64_t bar_full[NS], bar_empty[NS], bar_tile[kTileRing], bar_q[2], bar_s[2], bar_p[2], bar_o[2];
+  __shared__ TileWork s_tile[kTileRing];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_fail;
+
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  if (warp == kMmaWarpT) {
+    tmem_alloc(&s_tmem, 512);
+    tmem_relinquish();
+  }
+  if (tid == 0) {
+    for (int i = 0; i < NS; i++) {
+      mbar_init(&bar_full[i], 1);
+      mbar_init(&bar_empty[i], 1);
+    }
+    for (int i = 0; i < kTileRing; i++) mbar_init(&bar_tile[i], 1);
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&bar_q[i], 4);
+      mbar_init(&bar_s[i], 1);
+      mbar_init(&bar_p[i], 4);
+      mbar_init(&bar_o[i], 1);
+    }
+    mbar_fence_init();
+    s_fail = 0;
+    tma_prefetch_desc(&map_k);
+    tma_prefetch_desc(&map_v);
+  }
+  zero_rest<T, D>(p, blockIdx.x * kTileThreads + tid, gridDim.x * kTileThreads);
+  long long begin, end, units;
+  int shares;
+  Place at;
+  find_share<kTileThreads>(p, kTileRows, reinterpret_cast<long long*>(s_ring), begin, end, units, shares, at);
+  if (tid == 0 && blockIdx.x == 0) p.starts[p.max_shares] = ShareStart{units, shares, 0, 0, 0, 0, 0};
+  if (tid == 0 && begin < end) p.starts[blockIdx.x] = share_start(p, kTileRows, begin, at);
+  fence_proxy_async_smem();                                  // the copies overwrite the search's words
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tbase = s_tmem;
+  const int n = (int)(end - begin);
+
+  if (warp == kLoadWarp) {
+    // ------------------------------------------------------------------ copies
+    bool ok = true, first_piece = true;
+    int issued = 0;                                          // tiles of K or V
+    auto load = [&](int i, const CUtensorMap* map, const int32_t* table, int key, int length, int head) {
+      const int slot = i % NS;
+      if (i >= NS) ok = __all_sync(0xffffffffu, mbar_wait(&bar_empty[slot], ((i / NS) - 1) & 1));
+      ok = ok && !__any_sync(0xffffffffu, *(volatile int*)&s_fail);
+      if (!ok) return;
+      if (lane == 0) mbar_arrive_expect_tx(&bar_full[slot], Shape::kTile);
+      __syncwarp();
+      load_tile<D>(p, s_ring + slot * Shape::kTile, map, &bar_full[slot], table, key, length, head, lane);
+      issued = i + 1;
+    };
+    int done = 0;
+    for (int t = 0; done < n && ok; t++) {
+      const long long blocks = at.w.blocks(at.tile);
+      const int here = (int)min(blocks - at.block, (long long)(n - done));
+      const int key0 = (int)(at.block * kBlockKeys), length = (int)at.w.length;
+      if (lane == 0) {
+        TileWork w;
+        const bool whole = at.block == 0 && here == blocks;
+        w.units = here, w.key = key0;
+        w.token = at.token, w.row = (int)(at.tile * kTileRows), w.rows = (int)min((long long)kTileRows, at.w.all_rows() - at.tile * kTileRows);
+        w.head = at.head, w.length = length, w.visible0 = p.causal ? (int)(at.w.length - at.w.tokens) : length;
+        w.flags = (whole ? kWhole : 0) | (first_piece ? kHead : 0);
+        s_tile[t % kTileRing] = w;
+        mbar_arrive(&bar_tile[t % kTileRing]);
+      }
+      const int32_t* table = p.table + at.seq * p.table_stride;
+      for (int j = 0; j < here && ok; j++) {
+        const int key = key0 + j * kBlockKeys, i = 2 * (done + j);
+        load(i, &map_k, table, key, length, at.head);
+        if (ok) load(i + 1, &map_v, table, key, length, at.head);
+      }
+      done += here;
+      first_piece = false;
+      if (done < n) next_tile(p, kTileRows, at);
+    }
+    if (!ok) {
+      if (lane == 0) {
+        paged_report(p.dev_status, SPARGE_DEV_TIMEOUT_PRODUCER);
+        *(volatile int*)&s_fail = SPARGE_DEV_TIMEOUT_PRODUCER;
+      }
+      for (int i = max(0, issued - NS); i < issued; i++) mbar_wait(&bar_full[i % NS], (i / NS) & 1);   // our own copies land first
+    }
+  } else if (warp == kMmaWarpT) {
+    // ------------------------------------------------------------------ products
+    constexpr uint32_t fmt = std::is_same<T, __half>::value ? 0 : 1;
+    constexpr uint32_t idesc_qk = make_idesc(1, fmt, fmt, 0, 0, 128, kBlockKeys);
+    constexpr uint32_t idesc_pv = make_idesc(1, fmt, fmt, 0, 1, 128, D);
+    const uint64_t qd = make_smem_desc(smem_u32(smem), 16, 1024, kSwizzle128B);
+    const uint64_t kd = make_smem_desc(smem_u32(s_ring), 16, 1024, kSwizzle128B);
+    const uint64_t vd = make_smem_desc(smem_u32(s_ring), kBlockKeys * 128, 1024, kSwizzle128B);
+    const bool leader = elect_one();
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity)) && !__any_sync(0xffffffffu, *(volatile int*)&s_fail);
+    };
+    int steps[2] = {0, 0};                                   // of each half so far
+    auto issue_qk = [&](int x, int slot) {
+      if (!leader) return;
+#pragma unroll
+      for (int k = 0; k < D / 16; k++) {
+        const uint64_t off = (k & 3) * 2 + (k >> 2) * (kBlockKeys * 128 >> 4);
+        mma_f16_ss(tbase + x * 128, qd + x * (Shape::kQ >> 4) + off, kd + slot * (Shape::kTile >> 4) + off, idesc_qk, k > 0);
+      }
+      tc_commit(&bar_s[x]);
+    };
+    int done = 0;
+    for (int t = 0; done < n && ok; t++) {
+      wait(&bar_tile[t % kTileRing], (t / kTileRing) & 1);
+      if (!ok) break;
+      const int here = s_tile[t % kTileRing].units, rows = s_tile[t % kTileRing].rows, length = s_tile[t % kTileRing].length;
+      const int key0 = s_tile[t % kTileRing].key, both = rows > 128 ? 2 : 1;
+      wait(&bar_q[0], t & 1);
+      wait(&bar_q[1], t & 1);
+      const int i0 = 2 * done;
+      wait(&bar_full[i0 % NS], (i0 / NS) & 1);
+      if (!ok) break;
+      tc_fence_after();
+      for (int x = 0; x < both; x++) issue_qk(x, i0 % NS);
+      if (leader) tc_commit(&bar_empty[i0 % NS]);
+      for (int j = 0; j < here && ok; j++) {
+        const int iv = 2 * (done + j) + 1, ik = iv + 1, vslot = iv % NS, key = key0 + j * kBlockKeys;
+        const bool more = j + 1 < here;
+        wait(&bar_full[vslot], (iv / NS) & 1);
+        if (!ok) break;
+        if (key + kBlockKeys > length) {
+          // What an earlier owner left behind the length in its last page may be anything, NaN too, and 0 x NaN is no 0.
+          for (int c = lane; c < (kBlockKeys - max(0, length - key)) * 8; c += 32) {
+#pragma unroll
+            for (int h = 0; h < D / 64; h++)
+              *reinterpret_cast<uint4*>(s_ring + vslot * Shape::kTile + h * (kBlockKeys * 128) + max(0, length - key) * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        for (int x = 0; x < both; x++) {
+          if (x == 0 && more) wait(&bar_full[ik % NS], (ik / NS) & 1);
+          wait(&bar_p[x], steps[x]++ & 1);
+          if (!ok) break;
+          tc_fence_after();
+          if (leader) {
+#pragma unroll
+            for (int k = 0; k < kBlockKeys / 16; k++)
+              mma_f16_ts(tbase + 256 + x * 128, tbase + x * 128 + k * 8, vd + vslot * (Shape::kTile >> 4) + k * (2048 >> 4), idesc_pv, j > 0 || k > 0);
+          }
+          if (more) issue_qk(x, ik % NS);
+          else if (leader) tc_commit(&bar_o[x]);
+        }
+        if (ok && leader) {
+          tc_commit(&bar_empty[vslot]);
+          if (more) tc_commit(&bar_empty[ik % NS]);
+        }
+      }
+      if (ok && both == 1 && leader) tc_commit(&bar_o[1]);
+      done += here;
+    }
+    if (!ok && lane == 0) {
+      paged_report(p.dev_status, SPARGE_DEV_TIMEOUT_MMA);
+      *(volatile int*)&s_fail = SPARGE_DEV_TIMEOUT_MMA;
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------------ softmax, epilogue
+    const int x = warp >> 2, local = (warp & 3) * 32 + lane;   // tile, row of it
+    const uint32_t tlane = (uint32_t)((warp & 3) * 32) << 16, tS = tbase + x * 128 + tlane, tO = tbase + 256 + x * 128 + tlane;
+    uint8_t* s_q = smem + x * Shape::kQ + local * 128;
+    const bool negate = p.scale_log2 < 0.f;                    // the maximum of the products is that of the scores for a positive factor
+    const float c = fmaxf(fabsf(p.scale_log2), 1e-30f);        // (0 times minus infinity would be no score)
+    auto failed = [&]() { return *(volatile int*)&s_fail != 0; };
+
+    // A row's queries, on their way while the tile before it ends.
+    auto load_q = [&](const TileWork& w) {
+      const int r = x * 128 + local, seq_row = w.row + r, tok = seq_row / p.group;
+      const T* src = reinterpret_cast<const T*>(p.q) + (long long)(w.token + tok) * p.q_token + (long long)(w.head * p.group + seq_row - tok * p.group) * p.q_head;
+      const uint32_t flip = negate ? 0x80008000u : 0u;
+      uint4 v[D / 8];
+#pragma unroll
+      for (int k = 0; k < D / 8; k++) v[k] = r < w.rows ? reinterpret_cast<const uint4*>(src)[k] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int k = 0; k < D / 8; k++)
+        *reinterpret_cast<uint4*>(s_q + (k >> 3) * (128 * 128) + (((k & 7) ^ (local & 7)) << 4)) = make_uint4(v[k].x ^ flip, v[k].y ^ flip, v[k].z ^ flip, v[k].w ^ flip);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar_q[x]);
+    };
+
+    // Both halves go through every tile, one that has no rows in it too: nobody is more than a tile ahead of another, so that a
+    // barrier's parity names one phase.
+    int done = 0, t = 0, steps = 0;
+    TileWork w;
+    auto next_work = [&]() {
+      if (done >= n) return false;
+      mbar_wait_or_flag(&bar_tile[t % kTileRing], (t / kTileRing) & 1, &s_fail, SPARGE_DEV_TIMEOUT_SOFTMAX);
+      if (failed()) return false;
+      w = s_tile[t % kTileRing];
+      t++;
+      done += w.units;
+      if (w.rows > x * 128) load_q(w);
+      else if (lane == 0) mbar_arrive(&bar_q[x]);
+      return true;
+    };
+    bool have = next_work();
+    while (have) {
+      if (w.rows <= x * 128) {
+        mbar_wait_or_flag(&bar_o[x], (t - 1) & 1, &s_fail, SPARGE_DEV_TIMEOUT_SOFTMAX);
+        if (failed()) break;
+        have = next_work();
+        continue;
+      }
+      const int tile = t - 1;
+      const int r = x * 128 + local, seq_row = w.row + r, tok = seq_row / p.group;
+      const bool mine = r < w.rows, idle = x * 128 + (warp & 3) * 32 >= w.rows;   // no row of this warp is in the tile
+      const int limit = mine ? min(w.length, w.visible0 + (p.causal ? tok + 1 : 0)) : 0;
+      float m = -INFINITY, l = 0.f;
+      const int here = w.units, key0 = w.key;
+      for (int j = 0; j < here; j++) {
+        mbar_wait_or_flag(&bar_s[x], steps & 1, &s_fail, SPARGE_DEV_TIMEOUT_SOFTMAX);
+        steps++;
+        if (!idle) {
+          tc_fence_after();
+          uint32_t sr[128];
+          tmem_ld32(tS, sr);
+          tmem_ld32(tS + 32, sr + 32);
+          tmem_ld32(tS + 64, sr + 64);
+          tmem_ld32(tS + 96, sr + 96);
+          tmem_wait_ld();
+          float* s = reinterpret_cast<float*>(sr);
+          const int see = limit - (key0 + j * kBlockKeys);
+          if (__any_sync(0xffffffffu, see < kBlockKeys)) {
+#pragma unroll
+            for (int k = 0; k < kBlockKeys; k++) s[k] = k < see ? s[k] : -INFINITY;
+          }
+          float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+          for (int k = 4; k < kBlockKeys; k += 4) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) top[e] = fmaxf(top[e], s[k + e]);
+          }
+          const float mx = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), m);
+          if (__any_sync(0xffffffffu, (mx - m) * c > kRescaleFrom)) {   // (from minus infinity: always; both: NaN, never)
+            const float alpha = mx == -INFINITY ? 1.f : ex2_approx((m - mx) * c);
+            m = mx;
+            l *= alpha;
+            if (j > 0) {   // the products up to the step before are in O: S of this step came behind them
+#pragma unroll
+              for (int d = 0; d < D; d += 16) {
+                uint32_t ov[16];
+                tmem_ld16(tO + d, ov);
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 16; e++) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
+                tmem_st16(tO + d, ov);
+              }
+            }
+          }
+          float off = m == -INFINITY ? 0.f : -m * c;
+          // s c - m c in one rounding: what m c is off by is the same for the whole row, and goes out in the division. Where it
+          // could be off by whole powers of two the difference is taken first.
+          if (__any_sync(0xffffffffu, fabsf(off) > 1048576.f)) {
+#pragma unroll
+            for (int k = 0; k < kBlockKeys; k++) s[k] -= m == -INFINITY ? 0.f : m;
+            off = 0.f;
+          }
+          const float2 c2 = make_float2(c, c), off2 = make_float2(off, off);
+          float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int k0 = 0; k0 < kBlockKeys; k0 += 32) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int k = 0; k < 32; k += 4) {
+              float2 a = __ffma2_rn(make_float2(s[k0 + k], s[k0 + k + 1]), c2, off2);
+              float2 b = __ffma2_rn(make_float2(s[k0 + k + 2], s[k0 + k + 3]), c2, off2);
+              a = make_float2(ex2_approx(a.x), ex2_approx(a.y));
+              b = make_float2(ex2_approx(b.x), ex2_approx(b.y));
+              sum0 = __fadd2_rn(sum0, a);                   // the sum is of the unrounded values
+              sum1 = __fadd2_rn(sum1, b);
+              pk[k / 2] = pack_probs<T>(a.x, a.y);
+              pk[k / 2 + 1] = pack_probs<T>(b.x, b.y);
+            }
+            tmem_st16(tS + k0 / 2, pk);
+          }
+          sum0 = __fadd2_rn(sum0, sum1);
+          l += sum0.x + sum0.y;
+          tmem_wait_st();
+          tc_fence_before();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar_p[x]);
+        if (failed()) break;
+      }
+      const TileWork now = w;
+      have = next_work();                                    // S of this tile's last step is read: its queries are not needed any more
+      mbar_wait_or_flag(&bar_o[x], tile & 1, &s_fail, SPARGE_DEV_TIMEOUT_SOFTMAX);
+      if (failed()) break;
+      if (idle) continue;
+      tc_fence_after();
+      const bool whole = now.flags & kWhole;
+      const float inv = 1.f / l;
+      const int head = now.head * p.group + seq_row - tok * p.group;
+      T* dst = reinterpret_cast<T*>(p.out) + (long long)(now.token + tok) * p.out_token + (long long)head * p.out_head;
+      const long long part = ((long long)blockIdx.x * 2 + (now.flags & kHead ? 0 : 1)) * kTileRows + r;
+#pragma unroll
+      for (int d = 0; d < D; d += 32) {
+        uint32_t ov[32];
+        tmem_ld32(tO + d, ov);
+        tmem_wait_ld();
+        float* o = reinterpret_cast<float*>(ov);
+        if (mine && whole) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8)
+            *reinterpret_cast<uint4*>(dst + d + e) =
+                l != 0.f ? make_uint4(pack_probs<T>(o[e] * inv, o[e + 1] * inv), pack_probs<T>(o[e + 2] * inv, o[e + 3] * inv),
+                                     pack_probs<T>(o[e + 4] * inv, o[e + 5] * inv), pack_probs<T>(o[e + 6] * inv, o[e + 7] * inv))
+                        : make_uint4(0, 0, 0, 0);
+        } else if (mine) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(p.part_o + part * D + d + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        }
+      }
+      tc_fence_before();
+      if (mine && whole && p.lse)
+        p.lse[(long long)(now.token + tok) * (p.kv_heads * p.group) + head] = l != 0.f ? (m * c + log2f(l)) * 0.6931471805599453f : -INFINITY;
+      if (mine && !whole) p.part_ml[part * 2] = m == -INFINITY ? m : m * c, p.part_ml[part * 2 + 1] = l;
+    }
+    if (lane == 0 && failed()) paged_report(p.dev_status, SPARGE_DEV_TIMEOUT_SOFTMAX);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarpT) tmem_dealloc(tbase, 512);
+}
+
+template <typename T, int D>
+static int tile_launch(const PagedParams& p, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t st) {
+  auto kern = paged_tile_kernel<T, D>;
+  static std::atomic<uint64_t> done{0};
+  if (!kernel_attributes((const void*)kern, TileShape<D>::kSmemBytes, done)) return SPARGE_ERR_CUDA;
+  return launch(kern, dim3(p.max_shares), dim3(kTileThreads), TileShape<D>::kSmemBytes, st, false, k, v, p) == cudaSuccess ? SPARGE_OK : SPARGE_ERR_CUDA;
+}
+
+int paged_tile_launch(const PagedParams& p, const CUtensorMap& k, const CUtensorMap& v, int D, int dtype, cudaStream_t st) {
+  if (dtype == SPARGE_BF16) return D == 64 ? tile_launch<__nv_bfloat16, 64>(p, k, v, st) : tile_launch<__nv_bfloat16, 128>(p, k, v, st);
+  return D == 64 ? tile_launch<__half, 64>(p, k, v, st) : tile_launch<__half, 128>(p, k, v, st);
+}
+
+}  // namespace sparge

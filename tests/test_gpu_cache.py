@@ -271,6 +271,19 @@ def test_scales_and_extreme_scores(scale, chunk):
     assert (out.double() - mean).abs().max() <= 2 * 2.0 ** -8 * c["v_pages"][pages].transpose(0, 1).reshape(H, -1, D)[:, :400].float().abs().max()
 
 
+@pytest.mark.parametrize("chunk", [1, 150])
+def test_a_row_that_is_not_a_number_stays_one(chunk):
+    c = _make([300], 1, 64, 32, BF, 7)
+    q = torch.randn(chunk, 2, 64, generator=_gen(7)).to(BF).cuda()
+    cut = torch.tensor([0, chunk], dtype=torch.int32).cuda()
+    good = S.paged_attention(q, **c, cu_seqlens=cut, max_chunk=chunk)
+    q[chunk // 2, 1, 3] = math.nan
+    out, lse = S.paged_attention(q, **c, cu_seqlens=cut, max_chunk=chunk, return_lse=True)
+    assert out[chunk // 2, 1].isnan().all() and lse[chunk // 2, 1].isnan()
+    good[chunk // 2, 1] = out[chunk // 2, 1] = 0
+    assert torch.equal(out, good)
+
+
 @pytest.mark.parametrize("chunk", [1, 40])
 def test_bad_pages_are_reported_and_harmless(chunk):
     H, D = 2, 64
