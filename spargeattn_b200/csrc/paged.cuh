@@ -9,9 +9,10 @@
 
 namespace sparge {
 
-// A share's first tile, for the kernel that joins tiles which lie in several shares.
-struct ShareStart {
-  long long begin, first, last;   // the share's first unit; the tile's units [first, last)
+// The border between share c - 1 and share c, for the kernel that joins tiles which lie in several shares.
+struct ShareJoin {
+  int pieces;                     // of the tile around the border, in the shares c - 1, c, ...; 0: not the first border in a tile
+  int slot;                       // of the first piece; piece i > 0 has 2 (c - 1 + i)
   int token, row, rows, head;     // the sequence's first row of q; the tile's first row and their count; key head
 };
 
@@ -21,10 +22,10 @@ struct PagedParams {
   float* lse;
   long long q_token, q_head, out_token, out_head, table_stride;
   const int32_t *cu, *seq_lens, *table;
-  int tokens, sequences, width, num_pages, page_size, kv_heads, group;
+  int tokens, sequences, width, num_pages, page_size, page_shift, kv_heads, group;
   bool causal, zero_rest;
   float scale_log2;
-  ShareStart* starts;             // [shares + 1]: entry [shares] holds {units, shares, 0, ...}
+  ShareJoin* joins;               // [max_shares]
   float* part_o;                  // [shares][2][rows][D]: the share's first tile, its last one
   float* part_ml;                 // [shares][2][rows][2]
   int max_shares;
@@ -34,7 +35,7 @@ struct PagedParams {
 // What the loading warp tells the others about one unit.
 struct Unit {
   int flags;                      // kFirst, kLast: of the share's piece of a tile; kWhole: the piece is the tile; kHead: the share's first piece
-  int token, row, rows, head;     // as in ShareStart
+  int token, row, rows, head;     // as in ShareJoin
   int key;                        // the unit's first key
   int length;                     // keys of the sequence
   int visible0;                   // row r of the sequence sees min(length, visible0 + r / group + 1) keys
@@ -45,106 +46,115 @@ __device__ __forceinline__ void paged_report(int32_t* status, int code) {
   if (status) atomicCAS(status, 0, code);
 }
 
-__device__ __forceinline__ SeqWork load_seq(const PagedParams& p, int i, int rows, int& token) {
-  long long lo = i, hi = i + 1;
+template <int ROWS>
+__device__ __forceinline__ SeqWork<ROWS> load_seq(const PagedParams& p, int i, int& token) {
+  int lo = i, hi = i + 1;
   if (p.cu) {
     lo = max(0, min(p.cu[i], p.tokens));
-    hi = max((int)lo, min(p.cu[i + 1], p.tokens));
+    hi = max(lo, min(p.cu[i + 1], p.tokens));
   }
-  const long long most = (long long)p.width * p.page_size, len = p.seq_lens[i];
-  token = (int)lo;
-  return SeqWork{hi - lo, max(0LL, min(len, most)), p.group, rows, p.causal};
+  token = lo;
+  return SeqWork<ROWS>{(unsigned)(hi - lo), (unsigned)max(0, min(p.seq_lens[i], p.width << p.page_shift)), (unsigned)p.group, p.causal};
 }
 
 // A place on the line of units.
+template <int ROWS>
 struct Place {
   int seq, head, token;
-  long long tile, block, first;   // first: the tile's first unit
-  SeqWork w;
+  unsigned tile, block;
+  long long first;                // the tile's first unit
+  SeqWork<ROWS> w;
 };
 
-// Every thread of the CTA calls this. Returns the share's units [begin, end), and the place of its first one.
-// s: kThreads + 8 long longs of shared memory.
-template <int kThreads>
-__device__ __forceinline__ void find_share(const PagedParams& p, int rows, long long* s, long long& begin, long long& end,
-                                           long long& units, int& shares, Place& at) {
-  const int tid = threadIdx.x;
+// Every thread of the CTA calls this. Returns the share's units [begin, end), and the place of its first one. What a launch
+// spends here it spends before anything is loaded, so there are two barriers, and most of the arithmetic is 32-bit (with 64-bit
+// divisions and a barrier for every step: 6.5 us, of 18 that a call over one short sequence took).
+struct ShareSearch {              // in shared memory
+  long long warp[32], left;
+  int seq, token;
+  unsigned tokens, length;
+  unsigned tile;
+};
+template <int kThreads, int ROWS>
+__device__ __forceinline__ void find_share(const PagedParams& p, ShareSearch& s, long long& begin, long long& end, long long& units,
+                                           int& shares, Place<ROWS>& at) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = (p.sequences + kThreads - 1) / kThreads, lo = min(tid * per, p.sequences), hi = min(lo + per, p.sequences);
   long long mine = 0;
+  SeqWork<ROWS> w = {};
+  int token = 0;
   for (int i = lo; i < hi; i++) {
-    int token;
-    const SeqWork w = load_seq(p, i, rows, token);
+    w = load_seq<ROWS>(p, i, token);
     mine += w.units() * p.kv_heads;
-    if (p.seq_lens[i] != w.length) paged_report(p.dev_status, SPARGE_DEV_BAD_PAGE);
+    if (p.seq_lens[i] != (int)w.length) paged_report(p.dev_status, SPARGE_DEV_BAD_PAGE);
   }
-  s[tid] = mine;
-  __syncthreads();
-  if (tid < 32) {   // prefix sums of the threads' sums
-    constexpr int kEach = (kThreads + 31) / 32;
-    long long part[kEach], sum = 0;
+  long long x = mine;
 #pragma unroll
-    for (int i = 0; i < kEach; i++) {
-      part[i] = sum;
-      if (tid * kEach + i < kThreads) sum += s[tid * kEach + i];
-    }
-    long long x = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, x, o);
-      if (tid >= o) x += y;
-    }
-#pragma unroll
-    for (int i = 0; i < kEach; i++)
-      if (tid * kEach + i < kThreads) s[tid * kEach + i] = x - sum + part[i];
-    if (tid == 31) s[kThreads] = x;
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
   }
+  if (lane == 31) s.warp[warp] = x;
+  if (tid == 0) s.tile = 0;
   __syncthreads();
-  units = s[kThreads];
-  shares = (int)min((long long)p.max_shares, units);
+  long long before = x - mine;
+  units = 0;
+#pragma unroll
+  for (int i = 0; i < kThreads / 32; i++) {
+    const long long v = s.warp[i];
+    if (i < warp) before += v;
+    units += v;
+  }
+  shares = units < p.max_shares ? (int)units : p.max_shares;
   const int c = blockIdx.x;
   begin = end = 0;
   if (c >= shares) return;
   begin = share_begin(c, units, shares), end = share_begin(c + 1, units, shares);
-  const long long before = s[tid];
   if (before <= begin && begin < before + mine) {
     long long left = begin - before;
-    for (int i = lo; i < hi; i++) {
-      int token;
-      const SeqWork w = load_seq(p, i, rows, token);
-      const long long n = w.units() * p.kv_heads;
-      if (left < n) {
-        s[kThreads + 1] = i;
-        s[kThreads + 2] = left;
-        break;
+    int i = hi - 1;               // w is the last one of the thread's, most often the only one
+    if (per > 1) {
+      for (i = lo; i < hi; i++) {
+        w = load_seq<ROWS>(p, i, token);
+        const long long n = w.units() * p.kv_heads;
+        if (left < n) break;
+        left -= n;
       }
-      left -= n;
     }
+    s.seq = i, s.left = left, s.token = token, s.tokens = w.tokens, s.length = w.length;
   }
-  if (tid == 0) s[kThreads + 3] = 0;
   __syncthreads();
-  at.seq = (int)s[kThreads + 1];
-  long long left = s[kThreads + 2];
-  at.w = load_seq(p, at.seq, rows, at.token);
-  const long long per_head = at.w.units(), tiles = at.w.tiles();
-  at.head = (int)(left / per_head);
-  left -= at.head * per_head;
-  // the last tile that begins at or before the place: all threads try one each, then the gap between two of them
-  long long base = 0;
-  for (long long step = (tiles + kThreads - 1) / kThreads;; step = (step + kThreads - 1) / kThreads) {
-    const long long t = base + tid * step;
-    if (tiles > 1 && t < tiles && at.w.blocks_before(t) <= left) atomicMax(reinterpret_cast<unsigned long long*>(s + kThreads + 3), (unsigned long long)t);
-    __syncthreads();
-    base = s[kThreads + 3];
-    if (step <= 1) break;
-    __syncthreads();
+  at.seq = s.seq, at.token = s.token;
+  at.w = SeqWork<ROWS>{s.tokens, s.length, (unsigned)p.group, p.causal};
+  long long left = s.left;
+  const unsigned tiles = at.w.tiles();
+  if (tiles == 1) {
+    const unsigned blocks = at.w.blocks(0);
+    at.head = (int)((unsigned)left / blocks);          // heads times blocks of one sequence: below 2^31
+    at.tile = 0, at.block = (unsigned)left - at.head * blocks;
+  } else {
+    const long long per_head = at.w.units();
+    at.head = (int)(left / per_head);
+    left -= at.head * per_head;
+    // the last tile that begins at or before the place: all threads try one each, then the gap between two of them
+    unsigned base = 0;
+    for (unsigned step = (tiles + kThreads - 1) / kThreads;; step = (step + kThreads - 1) / kThreads) {
+      const unsigned t = base + tid * step;
+      if (t < tiles && at.w.blocks_before(t) <= left) atomicMax(&s.tile, t);
+      __syncthreads();
+      base = s.tile;
+      if (step <= 1) break;
+      __syncthreads();
+    }
+    at.tile = base;
+    at.block = (unsigned)(left - at.w.blocks_before(base));
   }
-  at.tile = base;
-  at.block = left - at.w.blocks_before(base);
   at.first = begin - at.block;
 }
 
 // The place of the tile behind this one, at its first block.
-__device__ __forceinline__ void next_tile(const PagedParams& p, int rows, Place& at) {
+template <int ROWS>
+__device__ __forceinline__ void next_tile(const PagedParams& p, Place<ROWS>& at) {
   at.first += at.w.blocks(at.tile);
   at.block = 0;
   if (++at.tile < at.w.tiles()) return;
@@ -154,13 +164,22 @@ __device__ __forceinline__ void next_tile(const PagedParams& p, int rows, Place&
   do {
     at.seq++;
     if (at.seq >= p.sequences) return;
-    at.w = load_seq(p, at.seq, rows, at.token);
+    at.w = load_seq<ROWS>(p, at.seq, at.token);
   } while (at.w.tokens == 0);
 }
 
-__device__ __forceinline__ ShareStart share_start(const PagedParams& p, int rows, long long begin, const Place& at) {
-  return ShareStart{begin, at.first, at.first + at.w.blocks(at.tile), at.token, (int)(at.tile * rows),
-                    (int)min((long long)rows, at.w.all_rows() - at.tile * rows), at.head};
+// What the joining kernel has to know of the border in front of this share. One thread of every CTA calls it.
+template <int ROWS>
+__device__ __forceinline__ void note_join(const PagedParams& p, long long begin, long long units, int shares, const Place<ROWS>& at) {
+  ShareJoin j = {};
+  const int c = blockIdx.x;
+  if (c < shares && begin > at.first) {
+    const long long before = share_begin(c - 1, units, shares), last = at.first + at.w.blocks(at.tile);
+    if (before <= at.first)
+      j = ShareJoin{share_of(last - 1, units, shares) - (c - 1) + 1, 2 * (c - 1) + (before < at.first), at.token, (int)(at.tile * ROWS),
+                    (int)at.w.tile_rows(at.tile), at.head};
+  }
+  p.joins[c] = j;
 }
 
 // Rows of q that belong to no sequence become zeros.
@@ -178,26 +197,20 @@ __device__ __forceinline__ void zero_rest(const PagedParams& p, int thread, int 
   }
 }
 
-// Key or value tile of a unit: kBlockKeys rows of D channels, in column halves of 64 (128 bytes, 128-byte swizzle). A copy
-// takes a page's rows of one half; keys that the sequence does not have, and pages that the pool does not have, are read
-// at a page number behind the last one, where the copy engine fills in zeros. So every tile is complete, and nothing of what
-// an earlier owner left behind in the tile's last pages is in it but the rest of the one page that the length ends in.
-template <int D>
-__device__ __forceinline__ void load_tile(const PagedParams& p, uint8_t* dst, const CUtensorMap* map, uint64_t* bar, const int32_t* table,
-                                          int key0, int length, int head, int lane) {
-  const int box = min(p.page_size, kBlockKeys), boxes = kBlockKeys / box;
-  if (lane < boxes * (D / 64)) {
-    const int half = lane / boxes, piece = lane - half * boxes, key = key0 + piece * box;
-    int page = p.num_pages;
-    if (key < length) {
-      page = table[key / p.page_size];
-      if (page < 0 || page >= p.num_pages) {
-        paged_report(p.dev_status, SPARGE_DEV_BAD_PAGE);
-        page = p.num_pages;
-      }
-    }
-    tma_load_4d(dst + half * (kBlockKeys * 128) + piece * box * 128, map, bar, half * 64, key & (p.page_size - 1), head, page);
-  }
+// Keys and values reach shared memory by the copy engine, a page's rows of one head at a time, in column halves of 64 (128 bytes,
+// 128-byte swizzle). Keys that the sequence does not have, and pages that the pool does not have, are read at a page number
+// behind the last one, where the copy engine fills in zeros. So every tile is complete, and nothing of what an earlier owner left
+// behind is in it but the rest of the one page that the length ends in.
+// A lane's entry of the table for a unit (the pages of its pieces, lane by lane), read while the unit before it is under way: a look
+// into the table just before each copy made the copies the slowest part of the kernel over long chunks (3 750 cycles a unit).
+__device__ __forceinline__ int table_entry(const PagedParams& p, int seq, int key, int length) {
+  return key < length ? p.table[seq * p.table_stride + (key >> p.page_shift)] : 0;
+}
+__device__ __forceinline__ int page_of(const PagedParams& p, int entry, int key, int length) {
+  if (key >= length) return p.num_pages;
+  if (entry >= 0 && entry < p.num_pages) return entry;
+  paged_report(p.dev_status, SPARGE_DEV_BAD_PAGE);
+  return p.num_pages;
 }
 
 int paged_decode_launch(const PagedParams& p, const CUtensorMap& k, const CUtensorMap& v, int D, int dtype, cudaStream_t st);

@@ -64,6 +64,20 @@ __device__ __forceinline__ uint32_t pack_pair<__nv_bfloat16>(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// Keys and values of a unit, a piece of up to 128 rows of one page after the other: [piece][half][rows][128 bytes]. A copy brings
+// both halves: with a copy for each, 2 KB of a 16-token page at a time, the copy engine was what bounded the kernel (4 150 cycles a
+// unit where HBM takes 2 850).
+template <int D>
+__device__ __forceinline__ void load_unit(const PagedParams& p, uint8_t* dst, const CUtensorMap* map_k, const CUtensorMap* map_v, uint64_t* bar,
+                                          int entry, int key0, int length, int head, int lane) {
+  const int box = min(p.page_size, kBlockKeys), boxes = kBlockKeys / box;
+  if (lane < 2 * boxes) {
+    const int of_v = lane >= boxes, piece = lane - of_v * boxes, key = key0 + piece * box;
+    tma_load_5d(dst + of_v * (kBlockKeys * D * 2) + piece * box * D * 2, of_v ? map_v : map_k, bar, 0, key & (p.page_size - 1), 0, head,
+                page_of(p, entry, key, length));
+  }
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kDecodeThreads, 1)
 paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PagedParams p) {
@@ -71,10 +85,11 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   constexpr int ST = Shape::kStages, R = kDecodeRows;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* s_o = reinterpret_cast<float*>(smem + ST * Shape::kStage);       // [warp][row][D]; first the search for the share
+  float* s_o = reinterpret_cast<float*>(smem + ST * Shape::kStage);       // [warp][row][D]
   __shared__ uint64_t bar_full[ST], bar_empty[ST], bar_join[2];
   __shared__ Unit s_unit[ST];
   __shared__ float s_ml[kDecodeWarps][R][2];
+  __shared__ ShareSearch s_search;
   __shared__ int s_fail;
 
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -93,47 +108,45 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   zero_rest<T, D>(p, blockIdx.x * kDecodeThreads + tid, gridDim.x * kDecodeThreads);
   long long begin, end, units;
   int shares;
-  Place at;
-  find_share<kDecodeThreads>(p, R, reinterpret_cast<long long*>(s_o), begin, end, units, shares, at);
-  if (tid == 0 && blockIdx.x == 0) p.starts[p.max_shares] = ShareStart{units, shares, 0, 0, 0, 0, 0};
+  Place<R> at;
+  find_share<kDecodeThreads>(p, s_search, begin, end, units, shares, at);
+  if (tid == 0) note_join(p, begin, units, shares, at);
   if (begin >= end) return;
-  if (tid == 0) p.starts[blockIdx.x] = share_start(p, R, begin, at);
-  __syncthreads();                                                        // barriers are set; the search's words are read
+  pdl_trigger();                                                          // the joining kernel's blocks may come and wait
 
   if (warp == kDecodeWarps) {
     // ------------------------------------------------------------------ loads
     const int n = (int)(end - begin);
+    const int box = min(p.page_size, kBlockKeys), piece_key = (lane & (kBlockKeys / box - 1)) * box;   // of this lane's copy
+    auto entry_at = [&]() { return table_entry(p, at.seq, (int)(at.block * kBlockKeys) + piece_key, (int)at.w.length); };
     bool ok = true, first_piece = true, fresh = true;
-    int issued = 0;
+    int issued = 0, entry = entry_at();
     for (int i = 0; i < n; i++) {
       const int slot = i % ST;
+      const unsigned blocks = at.w.blocks(at.tile);
+      const bool last = at.block + 1 == blocks || i + 1 == n;
+      const int key = (int)(at.block * kBlockKeys), length = (int)at.w.length, head = at.head;
+      Unit u;
+      const bool whole = at.first >= begin && at.first + blocks <= end;
+      u.flags = (fresh ? kFirst : 0) | (last ? kLast : 0) | (whole ? kWhole : 0) | (first_piece ? kHead : 0);
+      u.token = at.token, u.row = (int)(at.tile * R), u.rows = (int)at.w.tile_rows(at.tile), u.head = head;
+      u.key = key, u.length = length;
+      u.visible0 = p.causal ? length - (int)at.w.tokens : length;
+      fresh = last;
+      if (last) first_piece = false;
+      if (!last) at.block++;
+      else if (i + 1 < n) next_tile(p, at);
+      const int next = i + 1 < n ? entry_at() : 0;
       if (i >= ST) ok = __all_sync(0xffffffffu, mbar_wait(&bar_empty[slot], ((i / ST) - 1) & 1));
       if (!ok || __any_sync(0xffffffffu, *(volatile int*)&s_fail)) break;
-      const long long blocks = at.w.blocks(at.tile);
-      const bool last = at.block + 1 == blocks || i + 1 == n;
-      const int key = (int)(at.block * kBlockKeys), length = (int)at.w.length;
       if (lane == 0) {
-        Unit u;
-        const bool whole = at.first >= begin && at.first + blocks <= end;
-        u.flags = (fresh ? kFirst : 0) | (last ? kLast : 0) | (whole ? kWhole : 0) | (first_piece ? kHead : 0);
-        u.token = at.token, u.row = (int)(at.tile * R), u.rows = (int)min((long long)R, at.w.all_rows() - at.tile * R), u.head = at.head;
-        u.key = key, u.length = length;
-        u.visible0 = p.causal ? (int)(at.w.length - at.w.tokens) : length;
         s_unit[slot] = u;
         mbar_arrive_expect_tx(&bar_full[slot], Shape::kStage);
       }
       __syncwarp();
-      const int32_t* table = p.table + at.seq * p.table_stride;
-      load_tile<D>(p, smem + slot * Shape::kStage, &map_k, &bar_full[slot], table, key, length, at.head, lane);
-      load_tile<D>(p, smem + slot * Shape::kStage + Shape::kTile, &map_v, &bar_full[slot], table, key, length, at.head, lane);
+      load_unit<D>(p, smem + slot * Shape::kStage, &map_k, &map_v, &bar_full[slot], entry, key, length, head, lane);
       issued = i + 1;
-      fresh = false;
-      if (last) {
-        fresh = true, first_piece = false;
-        if (i + 1 < n) next_tile(p, R, at);
-      } else {
-        at.block++;
-      }
+      entry = next;
     }
     if (!ok && lane == 0) {
       paged_report(p.dev_status, SPARGE_DEV_TIMEOUT_PRODUCER);
@@ -151,6 +164,14 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   int limit[2];                                      // keys that the rows see
   int joins = 0;
   const int n = (int)(end - begin);
+  // where the warp's keys lie in a tile: rows of a piece of a page are together
+  const int box = min(p.page_size, kBlockKeys), half_bytes = box * 128;
+  auto row_at = [&](int row) { return (row & ~(box - 1)) * (D * 2) + (row & (box - 1)) * 128; };
+  uint32_t k_at[kWarpKeys / 8], v_at[kWarpKeys / 16];
+#pragma unroll
+  for (int t = 0; t < kWarpKeys / 8; t++) k_at[t] = row_at(warp * kWarpKeys + t * 8 + (lane & 7));
+#pragma unroll
+  for (int t = 0; t < kWarpKeys / 16; t++) v_at[t] = row_at(warp * kWarpKeys + t * 16 + (lane & 15));
   for (int i = 0; i < n; i++) {
     const int slot = i % ST;
     mbar_wait_or_flag(&bar_full[slot], (i / ST) & 1, &s_fail, SPARGE_DEV_TIMEOUT_SOFTMAX);
@@ -183,9 +204,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       for (int k = 0; k < D / 32; k++) {
 #pragma unroll
         for (int t = 0; t < kWarpKeys / 8; t++) {
-          const int row = warp * kWarpKeys + t * 8 + (lane & 7), chunk = (k & 1) * 4 + (lane >> 3);
+          const int chunk = (k & 1) * 4 + (lane >> 3);
           uint32_t b[4];
-          ldmatrix_x4<false>(b, sk + (k >> 1) * (kBlockKeys * 128) + row * 128 + ((chunk ^ (row & 7)) << 4));
+          ldmatrix_x4<false>(b, sk + (k >> 1) * half_bytes + k_at[t] + ((chunk ^ (lane & 7)) << 4));
           mma_16816<T>(s[t], qf[2 * k], b[0], b[1]);
           mma_16816<T>(s[t], qf[2 * k + 1], b[2], b[3]);
         }
@@ -235,7 +256,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         for (int r = u.length - key0; r < kWarpKeys; r++) {
 #pragma unroll
           for (int h = 0; h < D / 64; h++)
-            *reinterpret_cast<uint32_t*>(smem + slot * Shape::kStage + Shape::kTile + h * (kBlockKeys * 128) + (warp * kWarpKeys + r) * 128 + lane * 4) = 0u;
+            *reinterpret_cast<uint32_t*>(smem + slot * Shape::kStage + Shape::kTile + h * half_bytes + row_at(warp * kWarpKeys + r) + lane * 4) = 0u;
         }
         fence_proxy_async_smem();                                   // the copy engine writes here next
         __syncwarp();
@@ -245,9 +266,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       for (int t = 0; t < kWarpKeys / 16; t++) {
 #pragma unroll
         for (int d = 0; d < D / 16; d++) {
-          const int row = warp * kWarpKeys + t * 16 + (lane & 15), chunk = (d & 3) * 2 + (lane >> 4);
+          const int chunk = (d & 3) * 2 + (lane >> 4);
           uint32_t b[4];
-          ldmatrix_x4<true>(b, sv + (d >> 2) * (kBlockKeys * 128) + row * 128 + ((chunk ^ (row & 7)) << 4));
+          ldmatrix_x4<true>(b, sv + (d >> 2) * half_bytes + v_at[t] + ((chunk ^ (lane & 7)) << 4));
           mma_16816<T>(o[2 * d], pf[t], b[0], b[1]);
           mma_16816<T>(o[2 * d + 1], pf[t], b[2], b[3]);
         }

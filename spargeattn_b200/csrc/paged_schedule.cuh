@@ -19,10 +19,10 @@ namespace sparge {
 
 constexpr int kBlockKeys = 128;
 
-// sum over i in [0, n) of floor((a + b i) / m), for a, b >= 0, m > 0: the number of lattice points under a line, counted by
-// exchanging the axes as in Euclid's algorithm.
-SPARGE_SCHED long long floor_sum(long long n, long long a, long long b, long long m) {
-  long long sum = 0;
+// sum over i in [0, n) of floor((a + b i) / m), for m > 0: the number of lattice points under a line, counted by exchanging the
+// axes as in Euclid's algorithm.
+SPARGE_SCHED unsigned long long floor_sum(unsigned long long n, unsigned long long a, unsigned long long b, unsigned long long m) {
+  unsigned long long sum = 0;
   while (n > 0) {
     if (b >= m) {
       sum += n * (n - 1) / 2 * (b / m);
@@ -32,55 +32,69 @@ SPARGE_SCHED long long floor_sum(long long n, long long a, long long b, long lon
       sum += n * (a / m);
       a %= m;
     }
-    const long long top = a + b * n;
+    const unsigned long long top = a + b * n;
     if (top < m) break;
     n = top / m;
     a = top % m;
-    const long long t = b;
+    const unsigned long long t = b;
     b = m;
     m = t;
   }
   return sum;
 }
 
-// One sequence: its new tokens, its length with them, and the rows of a tile.
+// One sequence: its new tokens, its length with them, and the query heads of a key head. tokens * group and length are below 2^31.
+template <int ROWS>
 struct SeqWork {
-  long long tokens, length;
-  int group, rows;
+  unsigned tokens, length, group;
   bool causal;
 
-  SPARGE_SCHED long long all_rows() const { return tokens * group; }
-  SPARGE_SCHED long long tiles() const { return (all_rows() + rows - 1) / rows; }
+  SPARGE_SCHED unsigned all_rows() const { return tokens * group; }
+  SPARGE_SCHED unsigned tiles() const { return (all_rows() + ROWS - 1) / ROWS; }
+  SPARGE_SCHED unsigned tile_rows(unsigned tile) const {
+    const unsigned left = all_rows() - tile * ROWS;
+    return left < ROWS ? left : ROWS;
+  }
   // keys that row r sees; not above zero: none
-  SPARGE_SCHED long long visible(long long r) const { return causal ? length - tokens + r / group + 1 : length; }
-  SPARGE_SCHED long long last_row(long long tile) const {
-    const long long end = (tile + 1) * rows, all = all_rows();
-    return (end < all ? end : all) - 1;
+  SPARGE_SCHED int visible(unsigned r) const {
+    return causal ? (int)length - (int)tokens + (tokens == 1 ? 1 : (int)(r / group) + 1) : (int)length;
   }
   // blocks of one tile; a tile that sees nothing has one all the same, which writes its zeros
-  SPARGE_SCHED long long blocks(long long tile) const {
-    const long long v = visible(last_row(tile));
-    return v <= kBlockKeys ? 1 : (v + kBlockKeys - 1) / kBlockKeys;
+  SPARGE_SCHED unsigned blocks(unsigned tile) const {
+    const int v = visible(tile * ROWS + tile_rows(tile) - 1);
+    return v <= kBlockKeys ? 1u : ((unsigned)v + kBlockKeys - 1) / kBlockKeys;
   }
   // blocks of the tiles [0, t), t <= tiles()
-  SPARGE_SCHED long long blocks_before(long long t) const {
-    if (t <= 0) return 0;
-    if (!causal) return t * blocks(0);
-    const long long all = tiles();
-    if (t == all) return blocks_before(t - 1) + blocks(t - 1);
-    // blocks(i) = max(1, floor((a + b i) / m)) for every tile but the last: the floor of a floor is one floor
-    const long long m = (long long)kBlockKeys * group, a = group * (length - tokens + kBlockKeys) + rows - 1, b = rows;
-    long long first = 0;   // the tiles before it see one block or less
+  SPARGE_SCHED long long blocks_before(unsigned t) const {
+    if (t == 0) return 0;
+    if (!causal || tokens == 1) return (long long)t * blocks(0);
+    const unsigned all = tiles();
+    long long sum = 0;
+    if (t == all) {   // the last one may have fewer rows
+      sum = blocks(t - 1);
+      t--;
+    }
+    // blocks(i) = max(1, floor((a + b i) / m)) of the others: the floor of a floor is one floor
+    const long long m = (long long)kBlockKeys * group, b = ROWS;
+    long long a = (long long)group * ((long long)length - tokens + kBlockKeys) + ROWS - 1, first = 0;   // first: the tiles before it see one block or less
     if (a < m) {
       first = (m - a + b - 1) / b;
       if (first > t) first = t;
+      a += b * first;
     }
-    return first + floor_sum(t - first, a + b * first, b, m);
+    return sum + first + (t > first ? (long long)floor_sum(t - first, a, b, m) : 0);
   }
   SPARGE_SCHED long long units() const { return blocks_before(tiles()); }   // of one key head
 };
 
 // Where share c of `shares` begins on a line of `units`.
-SPARGE_SCHED long long share_begin(long long c, long long units, long long shares) { return c * units / shares; }
+SPARGE_SCHED long long share_begin(int c, long long units, int shares) {
+  const unsigned long long x = (unsigned long long)c * units;
+  return x >> 32 ? (long long)(x / (unsigned)shares) : (long long)((unsigned)x / (unsigned)shares);
+}
+// The share that a unit lies in: the last one that begins at or before it.
+SPARGE_SCHED int share_of(long long unit, long long units, int shares) {
+  return (int)(((unsigned long long)(unit + 1) * shares - 1) / (unsigned long long)units);
+}
 
 }  // namespace sparge

@@ -7,8 +7,8 @@
 // A CTA has two tiles of 128 rows (the rows of one key head: tokens by query heads of its group, so grouped heads share every
 // key that is fetched) and works on both in turn: while the softmax warps of one are busy, the tensor cores do P V and the next
 // Q K^T of the other. Their S, P and O fill tensor memory: columns [0, 128) S and P of the first, [128, 256) of the second,
-// [256, 384) and [384, 512) their outputs. 10 warps: 0-3 and 4-7 softmax and epilogue of a tile each, 8 the copies, 9 the
-// products. One CTA on each SM takes an equal run of the call's units (paged_schedule.cuh); the copies run ahead over the borders
+// [256, 384) and [384, 512) their outputs. 12 warps: 0-3 and 4-7 softmax and epilogue of a tile each, 8 the copies, 9 and
+// 10 the products of a tile each (11 completes a warpgroup, whose registers the softmax warps take over). One CTA on each SM takes an equal run of the call's units (paged_schedule.cuh); the copies run ahead over the borders
 // of tiles, heads and sequences, and a tile's queries are fetched while the last product of the tile before it is under way.
 //
 // The products of a step of 128 keys take 1 024 cycles for the two tiles at D = 128 and the exponentials as many (16 a cycle on
@@ -23,10 +23,12 @@
 
 namespace sparge {
 
-constexpr int kTileThreads = 320, kLoadWarp = 8, kMmaWarpT = 9;
+constexpr int kTileThreads = 384, kLoadWarp = 8, kMmaWarpT = 9;
+// Registers of a thread: the launch gives every one of the 384 the same 168; the softmax warps hold a row's 128 scores.
+constexpr int kSoftmaxRegs = 208, kOtherRegs = 80;
+static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs <= kTileThreads * 168, "more than the launch has");
 constexpr int kTileRing = 8;                     // tiles whose description may wait to be read
 constexpr float kRescaleFrom = 8.f;              // in log2
-
 template <int D>
 struct TileShape {
   static constexpr int kQ = 128 * D * 2;                       // one tile's queries
@@ -42,6 +44,12 @@ struct TileWork {
   int token, row, rows, head, length, visible0, flags;
 };
 
+template <int N, bool MORE>
+__device__ __forceinline__ void set_registers() {   // by whole warpgroups
+  if (MORE) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 // D[tmem] (+)= A[tmem] * B[smem], 16-bit inputs of one type, f32 accumulate, K = 16.
 __device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -50,6 +58,25 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uin
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
       "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
+}
+
+// The largest of a row's scores of a step: three-input maxima in four chains.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float row_max(const float* s) {
+  constexpr int kChain = kBlockKeys / 4;
+  float top[4];
+#pragma unroll
+  for (int g = 0; g < 4; g++) {
+    top[g] = max3(s[kChain * g], s[kChain * g + 1], s[kChain * g + 2]);
+#pragma unroll
+    for (int k = 3; k < kChain - 1; k += 2) top[g] = max3(top[g], s[kChain * g + k], s[kChain * g + k + 1]);
+    top[g] = fmaxf(top[g], s[kChain * g + kChain - 1]);
+  }
+  return fmaxf(max3(top[0], top[1], top[2]), top[3]);
 }
 
 template <typename T>
@@ -63,6 +90,17 @@ __device__ __forceinline__ uint32_t pack_probs(float a, float b) {
   }
 }
 
+// Key or value tile of a unit: [half][128 rows][128 bytes], as the products' descriptors want it.
+template <int D>
+__device__ __forceinline__ void load_tile(const PagedParams& p, uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int entry, int key0, int length, int head,
+                                          int lane) {
+  const int box = min(p.page_size, kBlockKeys), boxes = kBlockKeys / box;
+  if (lane < boxes * (D / 64)) {
+    const int half = lane / boxes, piece = lane - half * boxes, key = key0 + piece * box;
+    tma_load_5d(dst + half * (kBlockKeys * 128) + piece * box * 128, map, bar, 0, key & (p.page_size - 1), half, head, page_of(p, entry, key, length));
+  }
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kTileThreads, 1)
 paged_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PagedParams p) {
@@ -71,8 +109,9 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* s_ring = smem + 2 * Shape::kQ;
-  __shared__ uint64_t bar_full[NS], bar_empty[NS], bar_tile[kTileRing], bar_q[2], bar_s[2], bar_p[2], bar_o[2];
+  __shared__ uint64_t bar_full[NS], bar_empty[NS], bar_tile[kTileRing], bar_q[2], bar_s[2], bar_p[2][2], bar_o[2];
   __shared__ TileWork s_tile[kTileRing];
+  __shared__ ShareSearch s_search;
   __shared__ uint32_t s_tmem;
   __shared__ int s_fail;
 
@@ -90,7 +129,8 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     for (int i = 0; i < 2; i++) {
       mbar_init(&bar_q[i], 4);
       mbar_init(&bar_s[i], 1);
-      mbar_init(&bar_p[i], 4);
+      mbar_init(&bar_p[i][0], 4);
+      mbar_init(&bar_p[i][1], 4);
       mbar_init(&bar_o[i], 1);
     }
     mbar_fence_init();
@@ -101,55 +141,64 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   zero_rest<T, D>(p, blockIdx.x * kTileThreads + tid, gridDim.x * kTileThreads);
   long long begin, end, units;
   int shares;
-  Place at;
-  find_share<kTileThreads>(p, kTileRows, reinterpret_cast<long long*>(s_ring), begin, end, units, shares, at);
-  if (tid == 0 && blockIdx.x == 0) p.starts[p.max_shares] = ShareStart{units, shares, 0, 0, 0, 0, 0};
-  if (tid == 0 && begin < end) p.starts[blockIdx.x] = share_start(p, kTileRows, begin, at);
-  fence_proxy_async_smem();                                  // the copies overwrite the search's words
+  Place<kTileRows> at;
+  find_share<kTileThreads>(p, s_search, begin, end, units, shares, at);
+  if (tid == 0) note_join(p, begin, units, shares, at);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tbase = s_tmem;
   const int n = (int)(end - begin);
+  pdl_trigger();                                             // the joining kernel's blocks may come and wait
 
+  if (warp >= kLoadWarp) {
+  set_registers<kOtherRegs, false>();
   if (warp == kLoadWarp) {
     // ------------------------------------------------------------------ copies
+    const int box = min(p.page_size, kBlockKeys), piece_key = (lane & (kBlockKeys / box - 1)) * box;   // of this lane's copies
     bool ok = true, first_piece = true;
     int issued = 0;                                          // tiles of K or V
-    auto load = [&](int i, const CUtensorMap* map, const int32_t* table, int key, int length, int head) {
+    auto load = [&](int i, const CUtensorMap* map, int entry, int key, int length, int head) {
       const int slot = i % NS;
       if (i >= NS) ok = __all_sync(0xffffffffu, mbar_wait(&bar_empty[slot], ((i / NS) - 1) & 1));
       ok = ok && !__any_sync(0xffffffffu, *(volatile int*)&s_fail);
       if (!ok) return;
       if (lane == 0) mbar_arrive_expect_tx(&bar_full[slot], Shape::kTile);
       __syncwarp();
-      load_tile<D>(p, s_ring + slot * Shape::kTile, map, &bar_full[slot], table, key, length, head, lane);
+      load_tile<D>(p, s_ring + slot * Shape::kTile, map, &bar_full[slot], entry, key, length, head, lane);
       issued = i + 1;
     };
-    int done = 0;
+    auto entry_at = [&](int key) { return table_entry(p, at.seq, key + piece_key, (int)at.w.length); };
+    int done = 0, entry = n > 0 ? entry_at((int)(at.block * kBlockKeys)) : 0;
     for (int t = 0; done < n && ok; t++) {
-      const long long blocks = at.w.blocks(at.tile);
-      const int here = (int)min(blocks - at.block, (long long)(n - done));
-      const int key0 = (int)(at.block * kBlockKeys), length = (int)at.w.length;
+      const unsigned blocks = at.w.blocks(at.tile);
+      const int here = (int)min(blocks - at.block, (unsigned)(n - done));
+      const int key0 = (int)(at.block * kBlockKeys), length = (int)at.w.length, head = at.head;
       if (lane == 0) {
         TileWork w;
-        const bool whole = at.block == 0 && here == blocks;
+        const bool whole = at.block == 0 && here == (int)blocks;
         w.units = here, w.key = key0;
-        w.token = at.token, w.row = (int)(at.tile * kTileRows), w.rows = (int)min((long long)kTileRows, at.w.all_rows() - at.tile * kTileRows);
-        w.head = at.head, w.length = length, w.visible0 = p.causal ? (int)(at.w.length - at.w.tokens) : length;
+        w.token = at.token, w.row = (int)(at.tile * kTileRows), w.rows = (int)at.w.tile_rows(at.tile);
+        w.head = at.head, w.length = length, w.visible0 = p.causal ? length - (int)at.w.tokens : length;
         w.flags = (whole ? kWhole : 0) | (first_piece ? kHead : 0);
         s_tile[t % kTileRing] = w;
         mbar_arrive(&bar_tile[t % kTileRing]);
       }
-      const int32_t* table = p.table + at.seq * p.table_stride;
       for (int j = 0; j < here && ok; j++) {
         const int key = key0 + j * kBlockKeys, i = 2 * (done + j);
-        load(i, &map_k, table, key, length, at.head);
-        if (ok) load(i + 1, &map_v, table, key, length, at.head);
+        int next = 0;
+        if (j + 1 < here) {
+          next = entry_at(key + kBlockKeys);
+        } else if (done + here < n) {
+          next_tile(p, at);
+          next = entry_at(0);
+        }
+        load(i, &map_k, entry, key, length, head);
+        if (ok) load(i + 1, &map_v, entry, key, length, head);
+        entry = next;
       }
       done += here;
       first_piece = false;
-      if (done < n) next_tile(p, kTileRows, at);
     }
     if (!ok) {
       if (lane == 0) {
@@ -167,77 +216,94 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     const uint64_t kd = make_smem_desc(smem_u32(s_ring), 16, 1024, kSwizzle128B);
     const uint64_t vd = make_smem_desc(smem_u32(s_ring), kBlockKeys * 128, 1024, kSwizzle128B);
     const bool leader = elect_one();
-    bool ok = true;
-    auto wait = [&](uint64_t* bar, uint32_t parity) {
-      ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity)) && !__any_sync(0xffffffffu, *(volatile int*)&s_fail);
-    };
-    int steps[2] = {0, 0};                                   // of each half so far
-    auto issue_qk = [&](int x, int slot) {
-      if (!leader) return;
+    // Waits record a failure and run on, on whatever is there: the loop ends with its tile. With votes on the outcome of every
+    // wait the way of every product through this warp was what bounded the kernel.
+    auto wait = [&](uint64_t* bar, uint32_t parity) { mbar_wait_or_flag(bar, parity, &s_fail, SPARGE_DEV_TIMEOUT_MMA); };
+    auto issue_qk = [&](int x, uint64_t kslot) {
+      if (leader) {
 #pragma unroll
-      for (int k = 0; k < D / 16; k++) {
-        const uint64_t off = (k & 3) * 2 + (k >> 2) * (kBlockKeys * 128 >> 4);
-        mma_f16_ss(tbase + x * 128, qd + x * (Shape::kQ >> 4) + off, kd + slot * (Shape::kTile >> 4) + off, idesc_qk, k > 0);
+        for (int k = 0; k < D / 16; k++) {
+          const uint64_t off = (k & 3) * 2 + (k >> 2) * (kBlockKeys * 128 >> 4);
+          mma_f16_ss(tbase + x * 128, qd + x * (Shape::kQ >> 4) + off, kslot + off, idesc_qk, k > 0);
+        }
+        tc_commit(&bar_s[x]);
       }
-      tc_commit(&bar_s[x]);
     };
-    int done = 0;
-    for (int t = 0; done < n && ok; t++) {
+    int done = 0, steps[2] = {0, 0};                         // steps of each half so far
+    for (int t = 0; done < n; t++) {
       wait(&bar_tile[t % kTileRing], (t / kTileRing) & 1);
-      if (!ok) break;
+      if (*(volatile int*)&s_fail) break;
       const int here = s_tile[t % kTileRing].units, rows = s_tile[t % kTileRing].rows, length = s_tile[t % kTileRing].length;
-      const int key0 = s_tile[t % kTileRing].key, both = rows > 128 ? 2 : 1;
+      const int key0 = s_tile[t % kTileRing].key;
+      const bool both = rows > 128;
+      int islot = 2 * done % NS;                             // of the tile of K or V in hand
+      uint32_t iphase = (2 * done / NS) & 1;
+      auto step_slot = [&]() {
+        if (++islot == NS) islot = 0, iphase ^= 1;
+      };
       wait(&bar_q[0], t & 1);
       wait(&bar_q[1], t & 1);
-      const int i0 = 2 * done;
-      wait(&bar_full[i0 % NS], (i0 / NS) & 1);
-      if (!ok) break;
+      wait(&bar_full[islot], iphase);
       tc_fence_after();
-      for (int x = 0; x < both; x++) issue_qk(x, i0 % NS);
-      if (leader) tc_commit(&bar_empty[i0 % NS]);
-      for (int j = 0; j < here && ok; j++) {
-        const int iv = 2 * (done + j) + 1, ik = iv + 1, vslot = iv % NS, key = key0 + j * kBlockKeys;
+      const uint64_t first = kd + islot * (Shape::kTile >> 4);
+      issue_qk(0, first);
+      if (both) issue_qk(1, first);
+      if (leader) tc_commit(&bar_empty[islot]);
+      step_slot();
+      for (int j = 0; j < here; j++) {
         const bool more = j + 1 < here;
-        wait(&bar_full[vslot], (iv / NS) & 1);
-        if (!ok) break;
-        if (key + kBlockKeys > length) {
+        const int vslot = islot, behind = length - (key0 + j * kBlockKeys);
+        wait(&bar_full[islot], iphase);
+        step_slot();
+        const int kslot = islot;
+        if (more) {
+          wait(&bar_full[islot], iphase);
+          step_slot();
+        }
+        const uint64_t vt = vd + vslot * (Shape::kTile >> 4), kt = kd + kslot * (Shape::kTile >> 4);
+        if (behind < kBlockKeys) {
           // What an earlier owner left behind the length in its last page may be anything, NaN too, and 0 x NaN is no 0.
-          for (int c = lane; c < (kBlockKeys - max(0, length - key)) * 8; c += 32) {
+          const int from = max(0, behind);
+          for (int c = lane; c < (kBlockKeys - from) * 8; c += 32) {
 #pragma unroll
             for (int h = 0; h < D / 64; h++)
-              *reinterpret_cast<uint4*>(s_ring + vslot * Shape::kTile + h * (kBlockKeys * 128) + max(0, length - key) * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+              *reinterpret_cast<uint4*>(s_ring + vslot * Shape::kTile + h * (kBlockKeys * 128) + from * 128 + c * 16) = make_uint4(0, 0, 0, 0);
           }
           fence_proxy_async_smem();
           __syncwarp();
         }
-        for (int x = 0; x < both; x++) {
-          if (x == 0 && more) wait(&bar_full[ik % NS], (ik / NS) & 1);
-          wait(&bar_p[x], steps[x]++ & 1);
-          if (!ok) break;
-          tc_fence_after();
-          if (leader) {
+        auto half_step = [&](auto which) {
+          constexpr int x = decltype(which)::value;
 #pragma unroll
-            for (int k = 0; k < kBlockKeys / 16; k++)
-              mma_f16_ts(tbase + 256 + x * 128, tbase + x * 128 + k * 8, vd + vslot * (Shape::kTile >> 4) + k * (2048 >> 4), idesc_pv, j > 0 || k > 0);
+          for (int half = 0; half < 2; half++) {
+            wait(&bar_p[x][half], steps[x] & 1);
+            tc_fence_after();
+            if (leader) {
+#pragma unroll
+              for (int k = half * (kBlockKeys / 32); k < (half + 1) * (kBlockKeys / 32); k++)
+                mma_f16_ts(tbase + 256 + x * 128, tbase + x * 128 + k * 8, vt + k * (2048 >> 4), idesc_pv, j > 0 || k > 0);
+            }
           }
-          if (more) issue_qk(x, ik % NS);
+          steps[x]++;
+          if (more) issue_qk(x, kt);
           else if (leader) tc_commit(&bar_o[x]);
-        }
-        if (ok && leader) {
+        };
+        half_step(std::integral_constant<int, 0>());
+        if (both) half_step(std::integral_constant<int, 1>());
+        if (leader) {
           tc_commit(&bar_empty[vslot]);
-          if (more) tc_commit(&bar_empty[ik % NS]);
+          if (more) tc_commit(&bar_empty[kslot]);
         }
       }
-      if (ok && both == 1 && leader) tc_commit(&bar_o[1]);
+      if (!both && leader) tc_commit(&bar_o[1]);
       done += here;
     }
-    if (!ok && lane == 0) {
-      paged_report(p.dev_status, SPARGE_DEV_TIMEOUT_MMA);
-      *(volatile int*)&s_fail = SPARGE_DEV_TIMEOUT_MMA;
-    }
+    if (lane == 0 && *(volatile int*)&s_fail) paged_report(p.dev_status, SPARGE_DEV_TIMEOUT_MMA);
     __syncwarp();
+  }
   } else {
     // ------------------------------------------------------------------ softmax, epilogue
+    set_registers<kSoftmaxRegs, true>();
     const int x = warp >> 2, local = (warp & 3) * 32 + lane;   // tile, row of it
     const uint32_t tlane = (uint32_t)((warp & 3) * 32) << 16, tS = tbase + x * 128 + tlane, tO = tbase + 256 + x * 128 + tlane;
     uint8_t* s_q = smem + x * Shape::kQ + local * 128;
@@ -263,7 +329,8 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
 
     // Both halves go through every tile, one that has no rows in it too: nobody is more than a tile ahead of another, so that a
     // barrier's parity names one phase.
-    int done = 0, t = 0, steps = 0;
+    int done = 0, t = 0;
+    uint32_t phase = 0;                                        // parity of the next S
     TileWork w;
     auto next_work = [&]() {
       if (done >= n) return false;
@@ -291,11 +358,11 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       float m = -INFINITY, l = 0.f;
       const int here = w.units, key0 = w.key;
       for (int j = 0; j < here; j++) {
-        mbar_wait_or_flag(&bar_s[x], steps & 1, &s_fail, SPARGE_DEV_TIMEOUT_SOFTMAX);
-        steps++;
+        mbar_wait_or_flag(&bar_s[x], phase, &s_fail, SPARGE_DEV_TIMEOUT_SOFTMAX);
+        phase ^= 1;
         if (!idle) {
           tc_fence_after();
-          uint32_t sr[128];
+          uint32_t sr[kBlockKeys];
           tmem_ld32(tS, sr);
           tmem_ld32(tS + 32, sr + 32);
           tmem_ld32(tS + 64, sr + 64);
@@ -303,17 +370,12 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           tmem_wait_ld();
           float* s = reinterpret_cast<float*>(sr);
           const int see = limit - (key0 + j * kBlockKeys);
-          if (__any_sync(0xffffffffu, see < kBlockKeys)) {
+          const bool masked = __any_sync(0xffffffffu, see < kBlockKeys);
+          if (masked) {
 #pragma unroll
             for (int k = 0; k < kBlockKeys; k++) s[k] = k < see ? s[k] : -INFINITY;
           }
-          float top[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-          for (int k = 4; k < kBlockKeys; k += 4) {
-#pragma unroll
-            for (int e = 0; e < 4; e++) top[e] = fmaxf(top[e], s[k + e]);
-          }
-          const float mx = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), m);
+          const float mx = fmaxf(row_max(s), m);
           if (__any_sync(0xffffffffu, (mx - m) * c > kRescaleFrom)) {   // (from minus infinity: always; both: NaN, never)
             const float alpha = mx == -INFINITY ? 1.f : ex2_approx((m - mx) * c);
             m = mx;
@@ -330,9 +392,9 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
               }
             }
           }
-          float off = m == -INFINITY ? 0.f : -m * c;
           // s c - m c in one rounding: what m c is off by is the same for the whole row, and goes out in the division. Where it
           // could be off by whole powers of two the difference is taken first.
+          float off = m == -INFINITY ? 0.f : -m * c;
           if (__any_sync(0xffffffffu, fabsf(off) > 1048576.f)) {
 #pragma unroll
             for (int k = 0; k < kBlockKeys; k++) s[k] -= m == -INFINITY ? 0.f : m;
@@ -355,16 +417,22 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
               pk[k / 2 + 1] = pack_probs<T>(b.x, b.y);
             }
             tmem_st16(tS + k0 / 2, pk);
+            // The product with the first half of the keys begins under the exponentials of the second.
+            if (k0 & 32) {
+              tmem_wait_st();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&bar_p[x][k0 / 64]);
+            }
           }
           sum0 = __fadd2_rn(sum0, sum1);
           l += sum0.x + sum0.y;
-          tmem_wait_st();
-          tc_fence_before();
+        } else if (lane < 2) {
+          mbar_arrive(&bar_p[x][lane]);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bar_p[x]);
         if (failed()) break;
       }
+      if (failed()) break;
       const TileWork now = w;
       have = next_work();                                    // S of this tile's last step is read: its queries are not needed any more
       mbar_wait_or_flag(&bar_o[x], tile & 1, &s_fail, SPARGE_DEV_TIMEOUT_SOFTMAX);

@@ -140,35 +140,39 @@ def test_shares_of_attention(tmp_path):
 #include <initializer_list>
 #include "paged_schedule.cuh"
 using namespace sparge;
-int main() {
-  for (int group : {1, 2, 3, 5, 8, 12, 40, 128})
-    for (int rows : {16, 128, 256})
-      for (bool causal : {false, true})
-        for (long long tokens : {1, 2, 7, 16, 31, 100, 333, 1000})
-          for (long long length : {0, 1, 5, 100, 127, 128, 129, 333, 1000, 1001, 5003}) {
-            const SeqWork w{tokens, length, group, rows, causal};
-            long long sum = 0, all = 0;
-            for (long long t = 0; t < w.tiles(); t++) {
-              if (w.blocks_before(t) != sum || w.blocks(t) < 1) return 1;
-              sum += w.blocks(t);
-              // every key that a row of the tile sees lies in its blocks
-              for (long long r = t * rows; r <= w.last_row(t); r++) if (w.visible(r) > w.blocks(t) * kBlockKeys) return 2;
-              all += w.last_row(t) - t * rows + 1;
-            }
-            if (w.units() != sum || all != w.all_rows()) return 3;
+template <int ROWS>
+int check() {
+  for (unsigned group : {1, 2, 3, 5, 8, 12, 40, 128})
+    for (bool causal : {false, true})
+      for (unsigned tokens : {1, 2, 7, 16, 31, 100, 333, 1000})
+        for (unsigned length : {0, 1, 5, 100, 127, 128, 129, 333, 1000, 1001, 5003}) {
+          const SeqWork<ROWS> w{tokens, length, group, causal};
+          long long sum = 0, all = 0;
+          for (unsigned t = 0; t < w.tiles(); t++) {
+            if (w.blocks_before(t) != sum || w.blocks(t) < 1) return 1;
+            sum += w.blocks(t);
+            // every key that a row of the tile sees lies in its blocks
+            for (unsigned r = 0; r < w.tile_rows(t); r++)
+              if (w.visible(t * ROWS + r) > (long long)w.blocks(t) * kBlockKeys) return 2;
+            all += w.tile_rows(t);
           }
-  // lengths of a long context: no overflow
-  const SeqWork w{1 << 20, (1LL << 31) - 256, 8, 256, true};
+          if (w.units() != sum || all != w.all_rows()) return 3;
+        }
+  // a long context: no overflow
+  const SeqWork<ROWS> w{1u << 20, 0x7fffff00u, 8, true};
   long long sum = 0;
-  for (long long t = 0; t < w.tiles(); t++) sum += w.blocks(t);
-  if (w.units() != sum) return 4;
+  for (unsigned t = 0; t < w.tiles(); t++) sum += w.blocks(t);
+  return w.units() == sum ? 0 : 4;
+}
+int main() {
+  if (int rc = check<16>() + 10 * check<128>() + 100 * check<256>()) return rc;
   for (long long units : {1LL, 5LL, 147LL, 148LL, 1000LL, 12345678901LL})
-    for (long long shares : {1LL, 5LL, 148LL}) {
+    for (int shares : {1, 5, 148}) {
       if (shares > units) continue;
       long long at = 0, least = units, most = 0;
-      for (long long c = 0; c < shares; c++) {
+      for (int c = 0; c < shares; c++) {
         const long long a = share_begin(c, units, shares), b = share_begin(c + 1, units, shares);
-        if (a != at) return 5;
+        if (a != at || share_of(a, units, shares) != c || share_of(b - 1, units, shares) != c) return 5;
         at = b;
         least = b - a < least ? b - a : least, most = b - a > most ? b - a : most;
       }
