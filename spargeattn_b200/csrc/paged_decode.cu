@@ -105,6 +105,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     tma_prefetch_desc(&map_k);
     tma_prefetch_desc(&map_v);
   }
+  pdl_wait();                                                             // lengths, tables and queries come from the kernels before
+  pdl_trigger();                                                          // the joining kernel's blocks may come and wait
   zero_rest<T, D>(p, blockIdx.x * kDecodeThreads + tid, gridDim.x * kDecodeThreads);
   long long begin, end, units;
   int shares;
@@ -112,7 +114,6 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   find_share<kDecodeThreads>(p, s_search, begin, end, units, shares, at);
   if (tid == 0) note_join(p, begin, units, shares, at);
   if (begin >= end) return;
-  pdl_trigger();                                                          // the joining kernel's blocks may come and wait
 
   if (warp == kDecodeWarps) {
     // ------------------------------------------------------------------ loads
@@ -132,11 +133,6 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       u.token = at.token, u.row = (int)(at.tile * R), u.rows = (int)at.w.tile_rows(at.tile), u.head = head;
       u.key = key, u.length = length;
       u.visible0 = p.causal ? length - (int)at.w.tokens : length;
-      fresh = last;
-      if (last) first_piece = false;
-      if (!last) at.block++;
-      else if (i + 1 < n) next_tile(p, at);
-      const int next = i + 1 < n ? entry_at() : 0;
       if (i >= ST) ok = __all_sync(0xffffffffu, mbar_wait(&bar_empty[slot], ((i / ST) - 1) & 1));
       if (!ok || __any_sync(0xffffffffu, *(volatile int*)&s_fail)) break;
       if (lane == 0) {
@@ -146,7 +142,13 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       __syncwarp();
       load_unit<D>(p, smem + slot * Shape::kStage, &map_k, &map_v, &bar_full[slot], entry, key, length, head, lane);
       issued = i + 1;
-      entry = next;
+      fresh = last;
+      if (last) first_piece = false;
+      if (i + 1 < n) {
+        if (!last) at.block++;
+        else next_tile(p, at);
+        entry = entry_at();
+      }
     }
     if (!ok && lane == 0) {
       paged_report(p.dev_status, SPARGE_DEV_TIMEOUT_PRODUCER);
@@ -172,22 +174,30 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   for (int t = 0; t < kWarpKeys / 8; t++) k_at[t] = row_at(warp * kWarpKeys + t * 8 + (lane & 7));
 #pragma unroll
   for (int t = 0; t < kWarpKeys / 16; t++) v_at[t] = row_at(warp * kWarpKeys + t * 16 + (lane & 15));
+  auto load_q = [&](int token, int row, int rows, int kv_head) {
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+      const int r = g + 8 * x, seq_row = row + r, tok = seq_row / p.group;
+      const T* src = reinterpret_cast<const T*>(p.q) + (long long)(token + tok) * p.q_token + (long long)(kv_head * p.group + seq_row - tok * p.group) * p.q_head;
+#pragma unroll
+      for (int k = 0; k < D / 16; k++) {
+        qf[k][x] = r < rows ? *reinterpret_cast<const uint32_t*>(src + 16 * k + 2 * q4) : 0u;
+        qf[k][x + 2] = r < rows ? *reinterpret_cast<const uint32_t*>(src + 16 * k + 8 + 2 * q4) : 0u;
+      }
+    }
+  };
+  load_q(at.token, (int)(at.tile * R), (int)at.w.tile_rows(at.tile), at.head);
   for (int i = 0; i < n; i++) {
     const int slot = i % ST;
     mbar_wait_or_flag(&bar_full[slot], (i / ST) & 1, &s_fail, SPARGE_DEV_TIMEOUT_SOFTMAX);
     if (*(volatile int*)&s_fail) break;
     const Unit u = s_unit[slot];
     if (u.flags & kFirst) {
+      if (i > 0) load_q(u.token, u.row, u.rows, u.head);               // (the first tile's are under way)
 #pragma unroll
       for (int x = 0; x < 2; x++) {
-        const int r = g + 8 * x, seq_row = u.row + r, tok = seq_row / p.group;
-        limit[x] = r < u.rows ? min(u.length, u.visible0 + (p.causal ? tok + 1 : 0)) : 0;
-        const T* src = reinterpret_cast<const T*>(p.q) + (long long)(u.token + tok) * p.q_token + (long long)(u.head * p.group + seq_row - tok * p.group) * p.q_head;
-#pragma unroll
-        for (int k = 0; k < D / 16; k++) {
-          qf[k][x] = r < u.rows ? *reinterpret_cast<const uint32_t*>(src + 16 * k + 2 * q4) : 0u;
-          qf[k][x + 2] = r < u.rows ? *reinterpret_cast<const uint32_t*>(src + 16 * k + 8 + 2 * q4) : 0u;
-        }
+        const int r = g + 8 * x;
+        limit[x] = r < u.rows ? min(u.length, u.visible0 + (p.causal ? (u.row + r) / p.group + 1 : 0)) : 0;
         m[x] = -INFINITY, l[x] = 0.f;
       }
 #pragma unroll
@@ -342,7 +352,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar_join[1]);          // the parts are read: the next tile's may overwrite them
-      mbar_wait_or_flag(&bar_join[1], joins & 1, &s_fail, SPARGE_DEV_TIMEOUT_SOFTMAX);
+      if (i + 1 < n) mbar_wait_or_flag(&bar_join[1], joins & 1, &s_fail, SPARGE_DEV_TIMEOUT_SOFTMAX);
       joins++;
     }
   }
@@ -354,7 +364,7 @@ static int decode_launch(const PagedParams& p, const CUtensorMap& k, const CUten
   auto kern = paged_decode_kernel<T, D>;
   static std::atomic<uint64_t> done{0};
   if (!kernel_attributes((const void*)kern, DecodeShape<D>::kSmemBytes, done)) return SPARGE_ERR_CUDA;
-  return launch(kern, dim3(p.max_shares), dim3(kDecodeThreads), DecodeShape<D>::kSmemBytes, st, false, k, v, p) == cudaSuccess ? SPARGE_OK : SPARGE_ERR_CUDA;
+  return launch(kern, dim3(p.max_shares), dim3(kDecodeThreads), DecodeShape<D>::kSmemBytes, st, true, k, v, p) == cudaSuccess ? SPARGE_OK : SPARGE_ERR_CUDA;
 }
 
 int paged_decode_launch(const PagedParams& p, const CUtensorMap& k, const CUtensorMap& v, int D, int dtype, cudaStream_t st) {

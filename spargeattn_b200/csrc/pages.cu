@@ -104,6 +104,8 @@ __device__ __forceinline__ void report_page(int32_t* status, int code) {
 __global__ void __launch_bounds__(kPlanThreads) allocate_kernel(PageTable t, const int32_t* new_tokens, unsigned char* served,
                                                                 int32_t* list, int32_t* offset, int32_t* need) {
   __shared__ int s_scan[33];
+  pdl_wait();
+  pdl_trigger();
   const int tid = threadIdx.x;
   int total_need = 0;
   for (int base = 0; base < t.sequences; base += kPlanThreads) {
@@ -145,6 +147,8 @@ __global__ void __launch_bounds__(kPlanThreads) allocate_kernel(PageTable t, con
 // ------------------------------------------------------------------------------------------------------------- release
 // Every entry is taken out by an exchange: two blocks with the same sequence release each page once.
 __global__ void __launch_bounds__(256) free_kernel(PageTable t, const int32_t* which, int32_t* dev_status) {
+  pdl_wait();
+  pdl_trigger();
   const int s = which[blockIdx.x];
   if (s < 0 || s >= t.sequences) {
     if (s != -1 && threadIdx.x == 0) report_page(dev_status, SPARGE_DEV_BAD_PAGE);
@@ -186,6 +190,7 @@ __device__ __forceinline__ void copy_tasks(const PagePool& pool, int pairs, int 
 // A block per pair and slice of the pool, so that the search for its hazards is made once for all its copies.
 __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(PagePool pool, const int32_t* src, const int32_t* dst, int n, int pages,
                                                                   int32_t* dev_status) {
+  pdl_wait();
   const int i = blockIdx.x, from = src[i], to = dst[i];
   const bool outside = from < 0 || from >= pages || to < 0 || to >= pages;
   if (outside) {
@@ -211,18 +216,14 @@ struct ForkPlan {
   int32_t *state, *len, *at, *from, *to, *rows, *list;   // [n] each, rows [n][width], list [pages]
 };
 
-__global__ void __launch_bounds__(256) fork_gather_kernel(PageTable t, const int32_t* src, const int32_t* dst, int n, ForkPlan f,
-                                                          int32_t* dev_status) {
-  const int i = blockIdx.x, s = src[i], d = dst[i], tid = threadIdx.x;
+// Pair i by `threads` threads, of which this is number `tid`; later: whether a pair behind it has its destination.
+__device__ __forceinline__ void gather_pair(const PageTable& t, int i, int s, int d, bool later, const ForkPlan& f, int tid, int threads, int32_t* dev_status) {
   const bool inside = s >= 0 && s < t.sequences && d >= 0 && d < t.sequences;
-  int later = 0;
-  for (int j = i + 1 + tid; j < n; j += 256) later |= dst[j] == d;
-  later = __syncthreads_or(later);
   int state = !inside || later ? 0 : s == d ? 3 : 1;
   if (!inside && s != -1 && d != -1 && tid == 0) report_page(dev_status, SPARGE_DEV_BAD_PAGE);
   if (state == 1) {
     const int len = held_tokens(t, s), used = pages_of(len, t.page_size);
-    for (int e = tid; e < t.width; e += 256) f.rows[(long long)i * t.width + e] = e < used ? t.table[s * t.stride + e] : -1;
+    for (int e = tid; e < t.width; e += threads) f.rows[(long long)i * t.width + e] = e < used ? t.table[s * t.stride + e] : -1;
     if (len % t.page_size) {
       const int page = t.table[s * t.stride + used - 1];
       if (page >= 0 && page < t.pages) state = 2;
@@ -233,9 +234,34 @@ __global__ void __launch_bounds__(256) fork_gather_kernel(PageTable t, const int
   if (tid == 0) f.state[i] = state;
 }
 
-__global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(PageTable t, int n, ForkPlan f, unsigned char* served) {
+__global__ void __launch_bounds__(256) fork_gather_kernel(PageTable t, const int32_t* src, const int32_t* dst, int n, ForkPlan f,
+                                                          int32_t* dev_status) {
+  pdl_wait();
+  pdl_trigger();
+  const int i = blockIdx.x, d = dst[i];
+  int later = 0;
+  for (int j = i + 1 + threadIdx.x; j < n; j += 256) later |= dst[j] == d;
+  gather_pair(t, i, src[i], d, __syncthreads_or(later) != 0, f, threadIdx.x, 256, dev_status);
+}
+
+// GATHER: does what fork_gather_kernel does first, a warp for each pair. Where the rows are few that takes less than a launch: a
+// step of 16 forks, 32 pages wide, with what it releases and allocates 24 -> 17 us.
+template <bool GATHER>
+__global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(PageTable t, const int32_t* src, const int32_t* dst, int n, ForkPlan f,
+                                                                 unsigned char* served, int32_t* dev_status) {
   __shared__ int s_scan[33];
   pdl_wait();
+  pdl_trigger();
+  if (GATHER) {
+    const int lane = threadIdx.x & 31;
+    for (int i = threadIdx.x >> 5; i < n; i += kPlanThreads / 32) {
+      const int d = dst[i];
+      int later = 0;
+      for (int j = i + 1 + lane; j < n; j += 32) later |= dst[j] == d;
+      gather_pair(t, i, src[i], d, __any_sync(0xffffffffu, later), f, lane, 32, dev_status);
+    }
+    __syncthreads();
+  }
   int want = 0;
   for (int base = 0; base < n; base += kPlanThreads) {
     const int i = base + threadIdx.x;
@@ -290,6 +316,8 @@ __global__ void __launch_bounds__(kCopyThreads) fork_apply_kernel(PageTable t, c
 __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(int32_t* refs, int pages, int32_t* live, int32_t* moves,
                                                                     int32_t* list, int32_t* to) {
   __shared__ int s_scan[33];
+  pdl_wait();
+  pdl_trigger();
   const int count = collect(refs, pages, pages, (int32_t*)nullptr, s_scan, [](int, int c) { return c > 0; });
   const int n = collect(refs, pages, pages, list, s_scan, [=](int p, int c) { return (p < count) != (c > 0); }) / 2;
   for (int p = count + threadIdx.x; p < pages; p += kPlanThreads) to[p] = p;
@@ -351,8 +379,8 @@ extern "C" int sparge_allocate_pages(int32_t* page_table, int32_t* seq_lens, int
   if (sequences == 0) return SPARGE_OK;
   if ((table_width && !page_table) || !seq_lens || (num_pages && !ref_counts) || !new_tokens || !served || !workspace) return SPARGE_ERR_NULL;
   int32_t* w = (int32_t*)workspace;
-  allocate_kernel<<<1, kPlanThreads, 0, (cudaStream_t)stream>>>(t, new_tokens, served, w, w + num_pages, w + num_pages + sequences);
-  return launch_status();
+  return launch(allocate_kernel, dim3(1), dim3(kPlanThreads), 0, (cudaStream_t)stream, true, t, new_tokens, served, w, w + num_pages,
+                w + num_pages + sequences) == cudaSuccess ? SPARGE_OK : SPARGE_ERR_CUDA;
 }
 
 extern "C" int sparge_free_sequences(int32_t* page_table, int32_t* seq_lens, int32_t* ref_counts, const int32_t* which, int n,
@@ -363,8 +391,7 @@ extern "C" int sparge_free_sequences(int32_t* page_table, int32_t* seq_lens, int
   if (!table_ok(t) || n < 0) return SPARGE_ERR_INVALID_ARG;
   if (n == 0) return SPARGE_OK;
   if ((sequences && ((table_width && !page_table) || !seq_lens)) || (num_pages && !ref_counts) || !which) return SPARGE_ERR_NULL;
-  free_kernel<<<n, 256, 0, (cudaStream_t)stream>>>(t, which, dev_status);
-  return launch_status();
+  return launch(free_kernel, dim3(n), dim3(256), 0, (cudaStream_t)stream, true, t, which, dev_status) == cudaSuccess ? SPARGE_OK : SPARGE_ERR_CUDA;
 }
 
 extern "C" int sparge_fork_sequences(void* pages, long long outer, long long outer_bytes, long long page_stride_bytes, long long page_bytes,
@@ -381,9 +408,14 @@ extern "C" int sparge_fork_sequences(void* pages, long long outer, long long out
   int32_t* w = (int32_t*)workspace;
   const ForkPlan f{w, w + n, w + 2 * (size_t)n, w + 3 * (size_t)n, w + 4 * (size_t)n, w + 5 * (size_t)n + num_pages, w + 5 * (size_t)n};
   const cudaStream_t st = (cudaStream_t)stream;
-  fork_gather_kernel<<<n, 256, 0, st>>>(t, src, dst, n, f, dev_status);
-  if (int rc = launch_status()) return rc;
-  if (launch(fork_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, true, t, n, f, served) != cudaSuccess) return SPARGE_ERR_CUDA;
+  // one block reads and writes about 8 entries a cycle: up to 32 K of them cost it no more than the launch that they save
+  if ((long long)n * (table_width + n / 32) <= 32768) {
+    if (launch(fork_plan_kernel<true>, dim3(1), dim3(kPlanThreads), 0, st, true, t, src, dst, n, f, served, dev_status) != cudaSuccess) return SPARGE_ERR_CUDA;
+  } else {
+    if (launch(fork_gather_kernel, dim3(n), dim3(256), 0, st, true, t, src, dst, n, f, dev_status) != cudaSuccess ||
+        launch(fork_plan_kernel<false>, dim3(1), dim3(kPlanThreads), 0, st, true, t, src, dst, n, f, served, dev_status) != cudaSuccess)
+      return SPARGE_ERR_CUDA;
+  }
   if (launch(fork_apply_kernel, dim3(n + copy_blocks(pool, n)), dim3(kCopyThreads), 0, st, true, t, dst, n, f, pool) != cudaSuccess)
     return SPARGE_ERR_CUDA;
   return SPARGE_OK;
@@ -399,9 +431,8 @@ extern "C" int sparge_compact_pages(void* pages, long long outer, long long oute
   if (!live || !workspace || (num_pages && (!ref_counts || !pages)) || (sequences && table_width && !page_table)) return SPARGE_ERR_NULL;
   int32_t *list = (int32_t*)workspace, *to = list + num_pages, *moves = to + num_pages;
   const cudaStream_t st = (cudaStream_t)stream;
-  compact_plan_kernel<<<1, kPlanThreads, 0, st>>>(ref_counts, num_pages, live, moves, list, to);
-  if (int rc = launch_status()) return rc;
-  if (launch(compact_apply_kernel, dim3(copy_blocks(pool, num_pages / 2 + 1)), dim3(kCopyThreads), 0, st, true, pool, page_table, sequences, table_width,
+  if (launch(compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, true, ref_counts, num_pages, live, moves, list, to) != cudaSuccess ||
+      launch(compact_apply_kernel, dim3(copy_blocks(pool, num_pages / 2 + 1)), dim3(kCopyThreads), 0, st, true, pool, page_table, sequences, table_width,
              table_stride, num_pages, live, moves, list, to) != cudaSuccess)
     return SPARGE_ERR_CUDA;
   return SPARGE_OK;
@@ -416,6 +447,6 @@ extern "C" int sparge_copy_pages(void* pages, long long outer, long long outer_b
   if ((num_pages && !pages) || !src || !dst) return SPARGE_ERR_NULL;
   // one pair at a time fills the GPU only where pages are large or the pool has many slices
   const int slices = std::min(copy_blocks(pool, 1), std::max(1, 8 * sm_count() / n));
-  copy_pages_kernel<<<dim3(n, slices), kCopyThreads, 0, (cudaStream_t)stream>>>(pool, src, dst, n, num_pages, dev_status);
-  return launch_status();
+  return launch(copy_pages_kernel, dim3(n, slices), dim3(kCopyThreads), 0, (cudaStream_t)stream, true, pool, src, dst, n, num_pages, dev_status) == cudaSuccess
+             ? SPARGE_OK : SPARGE_ERR_CUDA;
 }

@@ -9,11 +9,16 @@
 // phase and its sine cost about 60 instructions, and a token's pairs are the same for all its heads: a block computes those of
 // its tokens once into shared memory, and a thread keeps the ones of its channels in registers while it walks the heads.
 #include "common.cuh"
+#include "launch.cuh"
 
 namespace sparge {
 
 constexpr int kRotThreads = 256;
 constexpr int kRotTokens = 8;      // most tokens of a block
+#ifndef AHEAD
+#define AHEAD 2
+#define RBLOCKS 4
+#endif
 
 struct RotSlot {                   // q, k or v
   const void* x;
@@ -80,14 +85,14 @@ struct Elem<float> {
   static __device__ __forceinline__ float from_float(float v) { return v; }
 };
 
-// The heads of one slot for one token: the thread's unit of channels, heads h0, h0 + step, ... Four heads are loaded before the
+// The heads of one slot for one token: the thread's unit of channels, heads h0, h0 + step, ... kAhead heads are loaded before the
 // first is turned: with one at a time the loads of a thread waited for one another.
-template <typename T, int V, bool VEC, bool INTER>
+template <typename T, int V, bool VEC, bool INTER, bool ROT>
 __device__ __forceinline__ void turn_heads(const T* x, T* y, long long xh, long long yh, int heads, int h0, int step, int unit,
                                            int rot_units, int pairs, const float2* cs, bool zero) {
   constexpr int P = INTER ? V / 2 : V;   // pairs of a unit
-  constexpr int kAhead = 4;
-  if (unit < rot_units) {
+  constexpr int kAhead = AHEAD;
+  if (ROT && unit < rot_units) {
     float2 c[P];
 #pragma unroll
     for (int i = 0; i < P; i++) c[i] = cs[unit * P + i];
@@ -151,13 +156,15 @@ __device__ __forceinline__ void turn_heads(const T* x, T* y, long long xh, long 
 }
 
 // V elements make a unit of the copied channels and half a unit of (i, i + pairs); VEC: 16-byte accesses.
-template <typename T, int V, bool VEC, bool INTER, bool PAGED>
-__global__ void __launch_bounds__(kRotThreads) rotary_kernel(const __grid_constant__ RotParams p) {
+template <typename T, int V, bool VEC, bool INTER, bool PAGED, bool ROT>
+__global__ void __launch_bounds__(kRotThreads, RBLOCKS) rotary_kernel(const __grid_constant__ RotParams p) {
   extern __shared__ float2 s_cs[];                  // [tokens_per_block][pairs]
   __shared__ int s_page[kRotTokens], s_row[kRotTokens], s_pos[kRotTokens];   // paged: -1 no page; row -1 behind the last sequence
   __shared__ int s_seq;
   const int tid = threadIdx.x, TOK = p.tokens_per_block;
   const long long tokens = (long long)p.B * p.N, t0 = (long long)blockIdx.x * TOK;
+  pdl_wait();
+  pdl_trigger();
 
   if (PAGED) {
     // the sequence of the block's first token: how many of them end at or before it
@@ -200,7 +207,7 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const __grid_consta
     __syncthreads();
   }
 
-  for (int i = tid; i < TOK * p.pairs; i += kRotThreads) {
+  for (int i = tid; ROT && i < TOK * p.pairs; i += kRotThreads) {
     const int tok = i / p.pairs, pair = i - tok * p.pairs;
     const long long t = t0 + tok;
     if (t >= tokens) break;
@@ -221,11 +228,11 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const __grid_consta
     sincospif((float)(2.0 * turn), &s, &c);
     s_cs[i] = make_float2(c * p.magnitude, (p.inverse ? -s : s) * p.magnitude);
   }
-  __syncthreads();
+  if (ROT) __syncthreads();
 
   for (int j = 0; j < p.slots; j++) {
     const RotSlot& sl = p.slot[j];
-    const int pairs = sl.rotate ? p.pairs : 0;
+    const int pairs = ROT && sl.rotate ? p.pairs : 0;
     const int rot_units = INTER ? 2 * pairs / V : pairs / V;
     const int units = rot_units + (p.D - 2 * pairs) / V;
     const int per = min(units, kRotThreads);           // threads of one token's head
@@ -247,12 +254,12 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const __grid_consta
         y += b * sl.yb + (t - (long long)b * p.N) * sl.yn;
       }
       for (int u = tid - group * per; u < units; u += per)
-        turn_heads<T, V, VEC, INTER>(x, y, sl.xh, sl.yh, sl.heads, h0, step, u, rot_units, pairs, s_cs + tok * p.pairs, zero);
+        turn_heads<T, V, VEC, INTER, ROT>(x, y, sl.xh, sl.yh, sl.heads, h0, step, u, rot_units, pairs, s_cs + tok * p.pairs, zero);
     }
   }
 }
 
-template <typename T, bool INTER, bool PAGED>
+template <typename T, bool INTER, bool PAGED, bool ROT>
 static int rotary_launch(RotParams& p, bool vec, cudaStream_t st) {
   const long long tokens = (long long)p.B * p.N;
   // Few tokens: a block each, so that a step's heads spread over the GPU; many: eight, whose angles share one pass.
@@ -260,9 +267,8 @@ static int rotary_launch(RotParams& p, bool vec, cudaStream_t st) {
   const size_t smem = sizeof(float2) * p.tokens_per_block * p.pairs;
   const long long blocks = (tokens + p.tokens_per_block - 1) / p.tokens_per_block;
   if (blocks > 0x7fffffffLL) return SPARGE_ERR_TOO_LARGE;
-  if (vec) rotary_kernel<T, 8, true, INTER, PAGED><<<(unsigned)blocks, kRotThreads, smem, st>>>(p);
-  else rotary_kernel<T, INTER ? 2 : 1, false, INTER, PAGED><<<(unsigned)blocks, kRotThreads, smem, st>>>(p);
-  return launch_status();
+  const auto kern = vec ? rotary_kernel<T, 8, true, INTER, PAGED, ROT> : rotary_kernel<T, INTER ? 2 : 1, false, INTER, PAGED, ROT>;
+  return launch(kern, dim3((unsigned)blocks), dim3(kRotThreads), smem, st, true, p) == cudaSuccess ? SPARGE_OK : SPARGE_ERR_CUDA;
 }
 
 // 16-byte accesses of 8 elements: the base, every stride and the channels' borders have to be multiples of them.
@@ -280,7 +286,9 @@ static bool vec_ok(const RotParams& p, bool inter, int elem) {
 template <bool PAGED>
 static int rotary_dispatch(RotParams& p, bool inter, int dtype, cudaStream_t st) {
   const bool vec = vec_ok(p, inter, dtype == SPARGE_F32 ? 4 : 2);
-#define SPARGE_ROT(T) (inter ? rotary_launch<T, true, PAGED>(p, vec, st) : rotary_launch<T, false, PAGED>(p, vec, st))
+#define SPARGE_ROT(T) \
+  (PAGED && p.pairs == 0 ? rotary_launch<T, false, PAGED, !PAGED>(p, vec, st) \
+                         : inter ? rotary_launch<T, true, PAGED, true>(p, vec, st) : rotary_launch<T, false, PAGED, true>(p, vec, st))
   if (dtype == SPARGE_BF16) return SPARGE_ROT(__nv_bfloat16);
   if (dtype == SPARGE_F16) return SPARGE_ROT(__half);
   if constexpr (!PAGED) return SPARGE_ROT(float);
