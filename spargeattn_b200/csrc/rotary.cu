@@ -15,10 +15,15 @@ namespace sparge {
 
 constexpr int kRotThreads = 256;
 constexpr int kRotTokens = 8;      // most tokens of a block
-#ifndef AHEAD
-#define AHEAD 2
-#define RBLOCKS 4
-#endif
+
+// What keeps HBM busy is blocks: six of them where the compiler needs no more registers than that (neighbouring pairs: 157 us for
+// the forward and backward pass of [1,12,32760,128] queries and keys, 174 with four), four where a unit has two halves (partial
+// rotation of [4097, 16 + 4, 128]: 12.1 us, 25.5 with six, which spill). Heads loaded together: more in flight and more registers
+// each (two against four: 157 and 183 us); without a rotation there is nothing else to hold, and four.
+template <bool INTER, bool ROT>
+struct RotShape {
+  static constexpr int kAhead = ROT ? 2 : 4, kBlocks = ROT && INTER ? 6 : 4;
+};
 
 struct RotSlot {                   // q, k or v
   const void* x;
@@ -85,31 +90,36 @@ struct Elem<float> {
   static __device__ __forceinline__ float from_float(float v) { return v; }
 };
 
-// The heads of one slot for one token: the thread's unit of channels, heads h0, h0 + step, ... kAhead heads are loaded before the
-// first is turned: with one at a time the loads of a thread waited for one another.
+// A unit of channels of kAhead heads, h, h + step, ...: loaded together, so that a thread does not wait for one head after the
+// other, then turned and stored. Units behind the rotated ones are copied as they are. zero: rows of no sequence.
 template <typename T, int V, bool VEC, bool INTER, bool ROT>
-__device__ __forceinline__ void turn_heads(const T* x, T* y, long long xh, long long yh, int heads, int h0, int step, int unit,
-                                           int rot_units, int pairs, const float2* cs, bool zero) {
-  constexpr int P = INTER ? V / 2 : V;   // pairs of a unit
-  constexpr int kAhead = AHEAD;
-  if (ROT && unit < rot_units) {
-    float2 c[P];
+struct HeadBatch {
+  static constexpr int kAhead = RotShape<INTER, ROT>::kAhead;
+  Raw<T, V> a[kAhead], b[kAhead];
+
+  __device__ __forceinline__ void load(const T* x, long long xh, int heads, int h, int step, int unit, int rot_units, int pairs, bool zero) {
+    const bool turn = ROT && unit < rot_units;
+    const int at = turn ? unit * V : 2 * pairs + (unit - rot_units) * V;
 #pragma unroll
-    for (int i = 0; i < P; i++) c[i] = cs[unit * P + i];
-    const int at = unit * V;
-    for (int h = h0; h < heads; h += kAhead * step) {
-      Raw<T, V> a[kAhead], b[kAhead];
+    for (int j = 0; j < kAhead; j++) {
+      const int hj = h + j * step;
+      if (hj < heads && !zero) {
+        a[j] = raw_load<T, V, VEC>(x + hj * xh + at);
+        if (!INTER && turn) b[j] = raw_load<T, V, VEC>(x + hj * xh + pairs + at);
+      } else {
 #pragma unroll
-      for (int j = 0; j < kAhead; j++) {
-        const int hj = h + j * step;
-        if (hj < heads && !zero) {
-          a[j] = raw_load<T, V, VEC>(x + hj * xh + at);
-          if (!INTER) b[j] = raw_load<T, V, VEC>(x + hj * xh + pairs + at);
-        } else {
-#pragma unroll
-          for (int i = 0; i < V; i++) a[j].v[i] = b[j].v[i] = Elem<T>::from_float(0.f);
-        }
+        for (int i = 0; i < V; i++) a[j].v[i] = b[j].v[i] = Elem<T>::from_float(0.f);
       }
+    }
+  }
+
+  __device__ __forceinline__ void store(T* y, long long yh, int heads, int h, int step, int unit, int rot_units, int pairs, const float2* cs) {
+    if (ROT && unit < rot_units) {
+      constexpr int P = INTER ? V / 2 : V;   // pairs of a unit
+      float2 c[P];
+#pragma unroll
+      for (int i = 0; i < P; i++) c[i] = cs[unit * P + i];
+      const int at = unit * V;
 #pragma unroll
       for (int j = 0; j < kAhead; j++) {
         const int hj = h + j * step;
@@ -132,20 +142,8 @@ __device__ __forceinline__ void turn_heads(const T* x, T* y, long long xh, long 
         }
         raw_store<T, V, VEC>(y + hj * yh + at, a[j]);
       }
-    }
-  } else {   // channels behind the rotated ones
-    const int at = 2 * pairs + (unit - rot_units) * V;
-    for (int h = h0; h < heads; h += kAhead * step) {
-      Raw<T, V> a[kAhead];
-#pragma unroll
-      for (int j = 0; j < kAhead; j++) {
-        const int hj = h + j * step;
-        if (hj < heads && !zero) a[j] = raw_load<T, V, VEC>(x + hj * xh + at);
-        else {
-#pragma unroll
-          for (int i = 0; i < V; i++) a[j].v[i] = Elem<T>::from_float(0.f);
-        }
-      }
+    } else {
+      const int at = 2 * pairs + (unit - rot_units) * V;
 #pragma unroll
       for (int j = 0; j < kAhead; j++) {
         const int hj = h + j * step;
@@ -153,11 +151,30 @@ __device__ __forceinline__ void turn_heads(const T* x, T* y, long long xh, long 
       }
     }
   }
+};
+
+// How a block's threads share a slot: `per` threads for a token's head, groups of them side by side over tokens, then heads.
+struct RotShare {
+  int pairs, rot_units, units, per, group, unit, step;
+  bool in;
+};
+template <int V, bool INTER, bool ROT>
+__device__ __forceinline__ RotShare rot_share(const RotParams& p, const RotSlot& sl, int tid) {
+  RotShare s;
+  s.pairs = ROT && sl.rotate ? p.pairs : 0;
+  s.rot_units = INTER ? 2 * s.pairs / V : s.pairs / V;
+  s.units = s.rot_units + (p.D - 2 * s.pairs) / V;
+  s.per = min(s.units, kRotThreads);
+  const int groups = kRotThreads / s.per;
+  s.group = tid / s.per, s.unit = tid - s.group * s.per;
+  s.step = max(1, groups / p.tokens_per_block);
+  s.in = s.group < groups;
+  return s;
 }
 
 // V elements make a unit of the copied channels and half a unit of (i, i + pairs); VEC: 16-byte accesses.
 template <typename T, int V, bool VEC, bool INTER, bool PAGED, bool ROT>
-__global__ void __launch_bounds__(kRotThreads, RBLOCKS) rotary_kernel(const __grid_constant__ RotParams p) {
+__global__ void __launch_bounds__(kRotThreads, (RotShape<INTER, ROT>::kBlocks)) rotary_kernel(const __grid_constant__ RotParams p) {
   extern __shared__ float2 s_cs[];                  // [tokens_per_block][pairs]
   __shared__ int s_page[kRotTokens], s_row[kRotTokens], s_pos[kRotTokens];   // paged: -1 no page; row -1 behind the last sequence
   __shared__ int s_seq;
@@ -207,6 +224,22 @@ __global__ void __launch_bounds__(kRotThreads, RBLOCKS) rotary_kernel(const __gr
     __syncthreads();
   }
 
+  // The first heads travel while the angles are computed.
+  HeadBatch<T, V, VEC, INTER, ROT> batch;
+  bool ahead = false;
+  if (!PAGED) {
+    const RotSlot& sl = p.slot[0];
+    const RotShare s = rot_share<V, INTER, ROT>(p, sl, tid);
+    const int tok = s.group % TOK, h0 = s.group / TOK;
+    const long long t = t0 + tok;
+    if (s.in && s.group < TOK * s.step && t < tokens && h0 < sl.heads) {
+      const int b = (int)(t / p.N);
+      batch.load(reinterpret_cast<const T*>(sl.x) + b * sl.xb + (t - (long long)b * p.N) * sl.xn, sl.xh, sl.heads, h0, s.step, s.unit, s.rot_units,
+                 s.pairs, false);
+      ahead = true;
+    }
+  }
+
   for (int i = tid; ROT && i < TOK * p.pairs; i += kRotThreads) {
     const int tok = i / p.pairs, pair = i - tok * p.pairs;
     const long long t = t0 + tok;
@@ -232,13 +265,9 @@ __global__ void __launch_bounds__(kRotThreads, RBLOCKS) rotary_kernel(const __gr
 
   for (int j = 0; j < p.slots; j++) {
     const RotSlot& sl = p.slot[j];
-    const int pairs = ROT && sl.rotate ? p.pairs : 0;
-    const int rot_units = INTER ? 2 * pairs / V : pairs / V;
-    const int units = rot_units + (p.D - 2 * pairs) / V;
-    const int per = min(units, kRotThreads);           // threads of one token's head
-    const int groups = kRotThreads / per, group = tid / per;
-    const int step = max(1, groups / TOK);             // heads side by side
-    for (int g = group; g < TOK * step && group < groups; g += groups) {
+    const RotShare s = rot_share<V, INTER, ROT>(p, sl, tid);
+    const int groups = kRotThreads / s.per;
+    for (int g = s.group; g < TOK * s.step && s.in; g += groups) {
       const int tok = g % TOK, h0 = g / TOK;
       const long long t = t0 + tok;
       if (t >= tokens) continue;
@@ -253,8 +282,13 @@ __global__ void __launch_bounds__(kRotThreads, RBLOCKS) rotary_kernel(const __gr
         zero = PAGED && s_row[tok] < 0;
         y += b * sl.yb + (t - (long long)b * p.N) * sl.yn;
       }
-      for (int u = tid - group * per; u < units; u += per)
-        turn_heads<T, V, VEC, INTER, ROT>(x, y, sl.xh, sl.yh, sl.heads, h0, step, u, rot_units, pairs, s_cs + tok * p.pairs, zero);
+      for (int u = s.unit; u < s.units; u += s.per) {
+        for (int h = h0; h < sl.heads; h += batch.kAhead * s.step) {
+          if (!ahead) batch.load(x, sl.xh, sl.heads, h, s.step, u, s.rot_units, s.pairs, zero);
+          ahead = false;
+          batch.store(y, sl.yh, sl.heads, h, s.step, u, s.rot_units, s.pairs, s_cs + tok * p.pairs);
+        }
+      }
     }
   }
 }
