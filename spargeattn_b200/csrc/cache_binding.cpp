@@ -6,6 +6,8 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -73,6 +75,18 @@ void check(int rc, const char* what) {
   TORCH_CHECK(false, what, ": ", text, " (status ", rc, ")");
 }
 sparge_stream_t stream_of(c10::Device dev) { return (sparge_stream_t)at::cuda::getCurrentCUDAStream(dev.index()).stream(); }
+// A contiguous tensor of the current stream's pool, and memory of it that lives for a call, without the dispatcher: a call of one
+// token takes the host as long as the GPU, and at::empty was a fifth of that each.
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, c10::Device dev) {
+  return at::detail::empty_cuda(sizes, type, dev, c10::nullopt);
+}
+Tensor fresh_like(const Tensor& t) {
+  if (t.is_contiguous()) return fresh(t.sizes(), t.scalar_type(), t.device());
+  const Tensor u = at::empty_like(t);                     // the storage order of a dense view
+  return u.stride(-1) == 1 ? u : at::empty(t.sizes(), t.options());
+}
+c10::DataPtr scratch(size_t bytes) { return c10::cuda::CUDACachingAllocator::get()->allocate(bytes); }
+
 int32_t* status_of(c10::Device dev) {
   Tensor* w = cache_status_word(dev.index());
   return w ? w->data_ptr<int32_t>() : nullptr;
@@ -165,14 +179,12 @@ PyObject* rotary_impl(PyObject* const* args, Py_ssize_t nargs) {
   };
   // the kernel reads any strides but a last dimension that is not dense
   const Tensor qc = q.stride(dim - 1) == 1 || D == 1 ? q : q.contiguous(), kc = !has_k || k.stride(dim - 1) == 1 ? k : k.contiguous();
-  Tensor qo = at::empty_like(qc), ko;
-  if (qo.stride(dim - 1) != 1) qo = at::empty(qc.sizes(), qc.options());
+  Tensor qo = fresh_like(qc), ko;
   a.B = (int)B, a.N = (int)N, a.D = (int)D, a.q_heads = (int)q.size(h);
   a.q = qc.data_ptr(), a.q_out = qo.data_ptr();
   strides(qc, a.q_st), strides(qo, a.q_out_st);
   if (has_k) {
-    ko = at::empty_like(kc);
-    if (ko.stride(dim - 1) != 1) ko = at::empty(kc.sizes(), kc.options());
+    ko = fresh_like(kc);
     a.k_heads = (int)k.size(h), a.k = kc.data_ptr(), a.k_out = ko.data_ptr();
     strides(kc, a.k_st), strides(ko, a.k_out_st);
   }
@@ -258,7 +270,7 @@ PyObject* append_impl(PyObject* const* args, Py_ssize_t nargs) {
   a.k = k.data_ptr(), a.v = v.data_ptr();
   a.k_st[0] = k.stride(0), a.k_st[1] = k.stride(1), a.v_st[0] = v.stride(0), a.v_st[1] = v.stride(1);
   if (q) {
-    qo = at::empty(q->sizes(), q->options());
+    qo = fresh(q->sizes(), q->scalar_type(), dev);
     a.q = q->data_ptr(), a.q_out = qo.data_ptr(), a.q_heads = (int)q->size(1);
     a.q_st[0] = q->stride(0), a.q_st[1] = q->stride(1), a.q_out_st[0] = qo.stride(0), a.q_out_st[1] = qo.stride(1);
   }
@@ -301,15 +313,15 @@ PyObject* attention_impl(PyObject* const* args, Py_ssize_t nargs) {
 
   const c10::cuda::CUDAGuard guard(dev);
   a.is_causal = truth(args[7]), a.scale = (float)scale, a.max_chunk = (int)chunk, a.q_heads = (int)q.size(1);
-  Tensor out = given ? *out_given : at::empty(q.sizes(), q.options()), lse;
+  Tensor out = given ? *out_given : fresh(q.sizes(), q.scalar_type(), dev), lse;
   if (want_lse) {
-    lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
+    lse = fresh({q.size(0), q.size(1)}, at::kFloat, dev);
     a.lse = lse.data_ptr<float>();
   }
   a.zero_rest = !given;
   a.workspace_bytes = sparge_paged_attention_workspace_bytes(a.q_heads, c.kv_heads, c.D, a.max_chunk);
-  Tensor ws = at::empty({(int64_t)a.workspace_bytes}, q.options().dtype(at::kByte));
-  a.workspace = ws.data_ptr();
+  const c10::DataPtr ws = scratch(a.workspace_bytes);
+  a.workspace = ws.get();
   a.q = q.data_ptr(), a.out = out.data_ptr();
   a.q_st[0] = q.stride(0), a.q_st[1] = q.stride(1), a.out_st[0] = out.stride(0), a.out_st[1] = out.stride(1);
   a.dev_status = status_of(dev);
@@ -386,9 +398,7 @@ PoolArgs pool_of(PyObject* o) {
        "pages must be 16-byte aligned");
   return p;
 }
-Tensor workspace(int n, int W, int P, c10::Device dev) {
-  return at::empty({(int64_t)sparge_pages_workspace_bytes(n, W, P)}, at::TensorOptions().dtype(at::kByte).device(dev));
-}
+c10::DataPtr workspace(int n, int W, int P) { return scratch(sparge_pages_workspace_bytes(n, W, P)); }
 
 // (page_table, seq_lens, ref_counts, new_tokens, page_size) -> served
 PyObject* allocate_impl(PyObject* const* args, Py_ssize_t nargs) {
@@ -400,8 +410,9 @@ PyObject* allocate_impl(PyObject* const* args, Py_ssize_t nargs) {
   const c10::Device dev = t.table->device();
   table_on_gpu(t, dev), on_gpu(more, dev, "new_tokens");
   const c10::cuda::CUDAGuard guard(dev);
-  Tensor served = at::empty({t.S}, at::TensorOptions().dtype(at::kBool).device(dev)), ws = workspace(t.S, 0, t.P, dev);
-  check(sparge_allocate_pages(t.pt, t.pl, t.pr, more.data_ptr<int32_t>(), (unsigned char*)served.data_ptr(), ws.data_ptr(), t.S, t.W,
+  Tensor served = fresh({t.S}, at::kBool, dev);
+  const c10::DataPtr ws = workspace(t.S, 0, t.P);
+  check(sparge_allocate_pages(t.pt, t.pl, t.pr, more.data_ptr<int32_t>(), (unsigned char*)served.data_ptr(), ws.get(), t.S, t.W,
                               t.table->stride(0), t.P, ps, stream_of(dev)), "allocate_pages");
   return THPVariable_Wrap(served);
 }
@@ -435,9 +446,10 @@ PyObject* fork_impl(PyObject* const* args, Py_ssize_t nargs) {
   const c10::Device dev = p.t->device();
   on_gpu(*p.t, dev, "pages"), table_on_gpu(t, dev), on_gpu(src, dev, "src"), on_gpu(dst, dev, "dst");
   const c10::cuda::CUDAGuard guard(dev);
-  Tensor served = at::empty({n}, at::TensorOptions().dtype(at::kBool).device(dev)), ws = workspace(n, t.W, t.P, dev);
+  Tensor served = fresh({n}, at::kBool, dev);
+  const c10::DataPtr ws = workspace(n, t.W, t.P);
   check(sparge_fork_sequences(p.t->data_ptr(), p.outer, p.outer_bytes, p.stride_bytes, p.page_bytes, t.pt, t.pl, t.pr, src.data_ptr<int32_t>(),
-                              dst.data_ptr<int32_t>(), (unsigned char*)served.data_ptr(), ws.data_ptr(), n, t.S, t.W, t.table->stride(0), t.P,
+                              dst.data_ptr<int32_t>(), (unsigned char*)served.data_ptr(), ws.get(), n, t.S, t.W, t.table->stride(0), t.P,
                               (int)p.page_size, status_of(dev), stream_of(dev)), "fork_sequences");
   return THPVariable_Wrap(served);
 }
@@ -451,9 +463,10 @@ PyObject* compact_impl(PyObject* const* args, Py_ssize_t nargs) {
   const c10::Device dev = p.t->device();
   on_gpu(*p.t, dev, "pages"), table_on_gpu(t, dev);
   const c10::cuda::CUDAGuard guard(dev);
-  Tensor live = at::empty({1}, at::TensorOptions().dtype(at::kInt).device(dev)), ws = workspace(0, 0, t.P, dev);
+  Tensor live = fresh({1}, at::kInt, dev);
+  const c10::DataPtr ws = workspace(0, 0, t.P);
   check(sparge_compact_pages(p.t->data_ptr(), p.outer, p.outer_bytes, p.stride_bytes, p.page_bytes, t.pt, t.pr, live.data_ptr<int32_t>(),
-                             ws.data_ptr(), t.S, t.W, t.table->stride(0), t.P, stream_of(dev)), "compact_pages");
+                             ws.get(), t.S, t.W, t.table->stride(0), t.P, stream_of(dev)), "compact_pages");
   return THPVariable_Wrap(live);
 }
 

@@ -112,7 +112,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* s_ring = smem + 2 * Shape::kQ;
-  __shared__ uint64_t bar_full[NS], bar_empty[NS], bar_tile[kTileRing], bar_q[2], bar_s[2], bar_p[2][kParts], bar_o[2];
+  __shared__ uint64_t bar_full[NS], bar_empty[NS], bar_tile[kTileRing], bar_q[2], bar_s[2], bar_p[2][kParts], bar_o[2], bar_end;
   __shared__ TileWork s_tile[kTileRing];
   __shared__ ShareSearch s_search;
   __shared__ uint32_t s_tmem;
@@ -129,6 +129,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       mbar_init(&bar_empty[i], 1);
     }
     for (int i = 0; i < kTileRing; i++) mbar_init(&bar_tile[i], 1);
+    mbar_init(&bar_end, 1);
     for (int i = 0; i < 2; i++) {
       mbar_init(&bar_q[i], 4);
       mbar_init(&bar_s[i], 1);
@@ -299,7 +300,10 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         if (!both && leader) tc_commit(&bar_o[1]);
         done += here;
       }
-      if (lane == 0 && *(volatile int*)&s_fail) paged_report(p.dev_status, SPARGE_DEV_TIMEOUT_MMA);
+      // every product, and every word about one, has arrived before the shared memory and the tensor memory go away
+      if (leader) tc_commit(&bar_end);
+      const bool ended = __all_sync(0xffffffffu, mbar_wait(&bar_end, 0));
+      if (lane == 0 && (!ended || *(volatile int*)&s_fail)) paged_report(p.dev_status, SPARGE_DEV_TIMEOUT_MMA);
       __syncwarp();
     }
   } else {
