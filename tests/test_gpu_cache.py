@@ -211,6 +211,44 @@ def test_chunks(Hq, Hkv, D, dtype, causal):
             _check_attention(o2, l2, q, c, lengths, cu, causal)
 
 
+# more sequences than threads of a CTA; some hold nothing, some bring nothing; one long one among them
+@pytest.mark.parametrize("sequences,most", [(700, 1), (700, 3), (1500, 40)])
+def test_many_sequences(sequences, most):
+    g = _gen(sequences + most)
+    H, D, ps = 2, 64, 16
+    chunks = [1] * sequences if most == 1 else torch.randint(0, most + 1, (sequences,), generator=g).tolist()
+    lengths = torch.randint(0, 90, (sequences,), generator=g).tolist()
+    lengths[sequences // 3] = 3000
+    c = _make(lengths, H, D, ps, HF, sequences)
+    cu = _cu(chunks)
+    q = torch.randn(cu[-1], 3 * H, D, generator=g).to(HF).cuda()
+    cut = None if most == 1 else torch.tensor(cu, dtype=torch.int32).cuda()
+    out, lse = S.paged_attention(q, **c, cu_seqlens=cut, max_chunk=most, return_lse=True)
+    _check_attention(out, lse, q, c, lengths, cu, True)
+
+
+@pytest.mark.parametrize("ps", [16, 256])
+@pytest.mark.parametrize("D,dtype", [(128, HF), (64, BF)])
+@pytest.mark.parametrize("Hq,Hkv", [(66, 33), (128, 1)])
+def test_chunks_of_many_heads(ps, D, dtype, Hq, Hkv):
+    chunks, lengths = [3, 17], [300, 1025]
+    c = _make(lengths, Hkv, D, ps, dtype, Hq + ps)
+    q = torch.randn(20, Hq, D, generator=_gen(19)).to(dtype).cuda()
+    for causal in (True, False):
+        out, lse = S.paged_attention(q, **c, cu_seqlens=torch.tensor([0, 3, 20], dtype=torch.int32).cuda(), max_chunk=17, is_causal=causal, return_lse=True)
+        _check_attention(out, lse, q, c, lengths, [0, 3, 20], causal)
+
+
+def test_output_over_the_queries():
+    """Every row of q is read before its output is written: out may be q itself."""
+    for chunk, length in ((1, 5000), (300, 2000)):
+        c = _make([length, 77], 1, 64, 16, BF, chunk)
+        q = torch.randn(2 * chunk, 4, 64, generator=_gen(20)).to(BF).cuda()
+        cut = torch.tensor([0, chunk, 2 * chunk], dtype=torch.int32).cuda()
+        want = S.paged_attention(q, **c, cu_seqlens=cut, max_chunk=chunk)
+        assert torch.equal(S.paged_attention(q, **c, cu_seqlens=cut, max_chunk=chunk, out=q), want) and torch.equal(q, want)
+
+
 @pytest.mark.parametrize("Hq,Hkv,chunk,length", [(8, 2, 3, 9001), (4, 1, 64, 20_000), (32, 4, 500, 2500), (2, 2, 1, 40_000)])
 def test_long_axis(Hq, Hkv, chunk, length):
     """Few rows over a long axis: many CTAs work on one tile and their parts are joined."""
@@ -475,6 +513,35 @@ def test_pool_runs_out():
     assert S.allocate_pages(table[:0], lens[:0], refs, empty, ps).shape == (0,)
 
 
+def test_captured_bookkeeping():
+    """Forks, growth, release and compaction in one graph, replayed over a pool that goes on changing."""
+    ps = 16
+    pages, table, lens, refs, o = _pool(300, ps, 12, 10, 21)
+    src, dst, new, gone = _i32(2, 3, 4), _i32(5, 6, 2), torch.full((12,), 3, dtype=torch.int32).cuda(), _i32(7, -1)
+    ops.device_status_word(pages.device)
+
+    def step():
+        S.fork_sequences(pages, table, lens, refs, src, dst)
+        served = S.allocate_pages(table, lens, refs, new, ps)
+        S.free_sequences(table, lens, refs, gone)
+        return served, S.compact_pages(pages, table, refs)
+
+    def want():
+        o.fork(src.tolist(), dst.tolist())
+        served = o.allocate(new.tolist())
+        o.free(gone.tolist())
+        return served, [o.compact()]
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        served, live = step()
+    for n in range(4):
+        graph.replay()
+        assert (served.tolist(), live.tolist()) == want()
+        _same(pages, table, lens, refs, o)
+        src.copy_(_i32(n, 8, 9)), dst.copy_(_i32(11, n + 1, 10)), gone.copy_(_i32(n + 4, n + 4))
+
+
 def test_copy_pages():
     g = _gen(13)
     for shape in ((2, 3, 9, 2, 16, 64), (40, 1, 16, 8), (3, 5, 4, 32, 128)):
@@ -644,16 +711,15 @@ def test_streams_and_threads():
         c = _make(lengths, Hkv, D, 32, BF, 100 + i)
         q = torch.randn(len(lengths) * chunk, Hq, D, generator=g).to(BF).cuda()
         cut = torch.tensor(_cu([chunk] * len(lengths)), dtype=torch.int32).cuda()
-        lens = [max(n, 0) for n in lengths]
-        work.append((c, q, cut, chunk, lens, S.paged_attention(q, **c, cu_seqlens=cut, max_chunk=chunk)))
+        work.append((c, q, cut, chunk, lengths, S.paged_attention(q, **c, cu_seqlens=cut, max_chunk=chunk)))
     torch.cuda.synchronize()
     wrong = []
 
-    def run(c, q, cut, chunk, lens, want):
+    def run(c, q, cut, chunk, lengths, want):
         with torch.cuda.stream(torch.cuda.Stream()):
             for _ in range(20):
                 if not torch.equal(S.paged_attention(q, **c, cu_seqlens=cut, max_chunk=chunk), want):
-                    wrong.append(lens)
+                    wrong.append(lengths)
 
     threads = [threading.Thread(target=run, args=w) for w in work for _ in range(2)]
     for t in threads:
