@@ -90,65 +90,45 @@ struct Elem<float> {
   static __device__ __forceinline__ float from_float(float v) { return v; }
 };
 
-// A unit of channels of kAhead heads, h, h + step, ...: loaded together, so that a thread does not wait for one head after the
-// other, then turned and stored. Units behind the rotated ones are copied as they are. zero: rows of no sequence.
+// A unit of channels of kAhead heads, a stride of dx (dy) elements apart, `left` of them there: loaded together, so that a thread
+// does not wait for one head after the other, then turned and stored. turn: else the unit lies behind the rotated channels and
+// is copied. The pointers walk: with an offset computed for every access the kernel was bound by its instructions.
 template <typename T, int V, bool VEC, bool INTER, bool ROT>
 struct HeadBatch {
-  static constexpr int kAhead = RotShape<INTER, ROT>::kAhead;
+  static constexpr int kAhead = RotShape<INTER, ROT>::kAhead, kPairs = INTER ? V / 2 : V;
   Raw<T, V> a[kAhead], b[kAhead];
 
-  __device__ __forceinline__ void load(const T* x, long long xh, int heads, int h, int step, int unit, int rot_units, int pairs, bool zero) {
-    const bool turn = ROT && unit < rot_units;
-    const int at = turn ? unit * V : 2 * pairs + (unit - rot_units) * V;
+  __device__ __forceinline__ void load(const T* x, long long dx, int left, int pairs, bool turn, bool zero) {
 #pragma unroll
     for (int j = 0; j < kAhead; j++) {
-      const int hj = h + j * step;
-      if (hj < heads && !zero) {
-        a[j] = raw_load<T, V, VEC>(x + hj * xh + at);
-        if (!INTER && turn) b[j] = raw_load<T, V, VEC>(x + hj * xh + pairs + at);
+      if (j < left && !zero) {
+        a[j] = raw_load<T, V, VEC>(x);
+        if (ROT && !INTER && turn) b[j] = raw_load<T, V, VEC>(x + pairs);
       } else {
 #pragma unroll
         for (int i = 0; i < V; i++) a[j].v[i] = b[j].v[i] = Elem<T>::from_float(0.f);
       }
+      x += dx;
     }
   }
 
-  __device__ __forceinline__ void store(T* y, long long yh, int heads, int h, int step, int unit, int rot_units, int pairs, const float2* cs) {
-    if (ROT && unit < rot_units) {
-      constexpr int P = INTER ? V / 2 : V;   // pairs of a unit
-      float2 c[P];
+  __device__ __forceinline__ void store(T* y, long long dy, int left, int pairs, bool turn, const float2* c) {
 #pragma unroll
-      for (int i = 0; i < P; i++) c[i] = cs[unit * P + i];
-      const int at = unit * V;
+    for (int j = 0; j < kAhead; j++) {
+      if (j >= left) break;
+      if (ROT && turn) {
 #pragma unroll
-      for (int j = 0; j < kAhead; j++) {
-        const int hj = h + j * step;
-        if (hj >= heads) break;
-        if (INTER) {
-#pragma unroll
-          for (int i = 0; i < P; i++) {
-            const float u = Elem<T>::to_float(a[j].v[2 * i]), w = Elem<T>::to_float(a[j].v[2 * i + 1]);
-            a[j].v[2 * i] = Elem<T>::from_float(u * c[i].x - w * c[i].y);
-            a[j].v[2 * i + 1] = Elem<T>::from_float(u * c[i].y + w * c[i].x);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < P; i++) {
-            const float u = Elem<T>::to_float(a[j].v[i]), w = Elem<T>::to_float(b[j].v[i]);
-            a[j].v[i] = Elem<T>::from_float(u * c[i].x - w * c[i].y);
-            b[j].v[i] = Elem<T>::from_float(u * c[i].y + w * c[i].x);
-          }
-          raw_store<T, V, VEC>(y + hj * yh + pairs + at, b[j]);
+        for (int i = 0; i < kPairs; i++) {
+          T& lo = INTER ? a[j].v[2 * i] : a[j].v[i];
+          T& hi = INTER ? a[j].v[2 * i + 1] : b[j].v[i];
+          const float u = Elem<T>::to_float(lo), w = Elem<T>::to_float(hi);
+          lo = Elem<T>::from_float(u * c[i].x - w * c[i].y);
+          hi = Elem<T>::from_float(u * c[i].y + w * c[i].x);
         }
-        raw_store<T, V, VEC>(y + hj * yh + at, a[j]);
+        if (!INTER) raw_store<T, V, VEC>(y + pairs, b[j]);
       }
-    } else {
-      const int at = 2 * pairs + (unit - rot_units) * V;
-#pragma unroll
-      for (int j = 0; j < kAhead; j++) {
-        const int hj = h + j * step;
-        if (hj < heads) raw_store<T, V, VEC>(y + hj * yh + at, a[j]);
-      }
+      raw_store<T, V, VEC>(y, a[j]);
+      y += dy;
     }
   }
 };
@@ -157,6 +137,7 @@ struct HeadBatch {
 struct RotShare {
   int pairs, rot_units, units, per, group, unit, step;
   bool in;
+  __device__ __forceinline__ int channel(int u, int v) const { return u < rot_units ? u * v : 2 * pairs + (u - rot_units) * v; }
 };
 template <int V, bool INTER, bool ROT>
 __device__ __forceinline__ RotShare rot_share(const RotParams& p, const RotSlot& sl, int tid) {
@@ -234,8 +215,9 @@ __global__ void __launch_bounds__(kRotThreads, (RotShape<INTER, ROT>::kBlocks)) 
     const long long t = t0 + tok;
     if (s.in && s.group < TOK * s.step && t < tokens && h0 < sl.heads) {
       const int b = (int)(t / p.N);
-      batch.load(reinterpret_cast<const T*>(sl.x) + b * sl.xb + (t - (long long)b * p.N) * sl.xn, sl.xh, sl.heads, h0, s.step, s.unit, s.rot_units,
-                 s.pairs, false);
+      const bool turn = s.unit < s.rot_units;
+      batch.load(reinterpret_cast<const T*>(sl.x) + b * sl.xb + (t - (long long)b * p.N) * sl.xn + h0 * sl.xh + s.channel(s.unit, V), s.step * sl.xh,
+                 (sl.heads - h0 + s.step - 1) / s.step, s.pairs, turn, false);
       ahead = true;
     }
   }
@@ -282,11 +264,21 @@ __global__ void __launch_bounds__(kRotThreads, (RotShape<INTER, ROT>::kBlocks)) 
         zero = PAGED && s_row[tok] < 0;
         y += b * sl.yb + (t - (long long)b * p.N) * sl.yn;
       }
+      const long long dx = s.step * sl.xh, dy = s.step * sl.yh;
       for (int u = s.unit; u < s.units; u += s.per) {
-        for (int h = h0; h < sl.heads; h += batch.kAhead * s.step) {
-          if (!ahead) batch.load(x, sl.xh, sl.heads, h, s.step, u, s.rot_units, s.pairs, zero);
+        const bool turn = u < s.rot_units;
+        float2 c[batch.kPairs];
+        if (ROT && turn) {
+#pragma unroll
+          for (int i = 0; i < batch.kPairs; i++) c[i] = s_cs[tok * p.pairs + u * batch.kPairs + i];
+        }
+        const T* px = x + h0 * sl.xh + s.channel(u, V);
+        T* py = y + h0 * sl.yh + s.channel(u, V);
+        for (int left = (sl.heads - h0 + s.step - 1) / s.step; left > 0; left -= batch.kAhead) {
+          if (!ahead) batch.load(px, dx, left, s.pairs, turn, zero);
           ahead = false;
-          batch.store(y, sl.yh, sl.heads, h, s.step, u, s.rot_units, s.pairs, s_cs + tok * p.pairs);
+          batch.store(py, dy, left, s.pairs, turn, c);
+          px += batch.kAhead * dx, py += batch.kAhead * dy;
         }
       }
     }

@@ -61,27 +61,6 @@ def rotary_frequencies(dim, base=10000.0, scaling=None, factor=1.0, original_len
     return f.to(device), magnitude
 
 
-class _Rotary(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, positions, frequencies, interleaved, sections, magnitude, layout):
-        ctx.save_for_backward(positions, frequencies)
-        ctx.how = interleaved, sections, magnitude, layout
-        return _binding.rotary(q, k, positions, frequencies, interleaved, sections, magnitude, layout, False)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dq, dk=None):
-        positions, frequencies = ctx.saved_tensors
-        interleaved, sections, magnitude, layout = ctx.how
-        turn = lambda a, b: _binding.rotary(a, b, positions, frequencies, interleaved, sections, magnitude, layout, True)  # noqa: E731
-        need_q, need_k = ctx.needs_input_grad[:2]
-        if need_q and need_k and dk is not None:
-            dq, dk = turn(dq, dk)
-        else:
-            dq, dk = turn(dq, None) if need_q else None, turn(dk, None) if need_k else None
-        return dq, dk, None, None, None, None, None, None
-
-
 @_skip_frame
 def apply_rotary(q, k, positions, frequencies, interleaved=False, sections=None, magnitude=1.0, tensor_layout="HND"):
     """Turns pairs of channels of q and k by position * frequency and returns (q', k'), or q' where k is None.
@@ -91,9 +70,7 @@ def apply_rotary(q, k, positions, frequencies, interleaved=False, sections=None,
     channels behind them are copied. `interleaved`: pairs are neighbours (2 i, 2 i + 1), else (i, i + pairs). `positions`: int32 or
     int64 [N] or [B, N]. With `sections` (pairs per axis, in order) positions have an axis of that length in front, and a
     pair turns by the position on its axis: frame, row and column of a video. Angles are formed in 64 bits, so far
-    positions lose nothing. Differentiable once, in q and k.
+    positions lose nothing. Differentiable in q and k; the gradient is turned back by the same kernel.
 
     Work is queued on the current stream. Shapes, types and ranges that do not fit are ValueError, CPU tensors RuntimeError."""
-    if torch.is_grad_enabled() and ((isinstance(q, torch.Tensor) and q.requires_grad) or (isinstance(k, torch.Tensor) and k.requires_grad)):
-        return _Rotary.apply(q, k, positions, frequencies, interleaved, sections, magnitude, tensor_layout)
-    return _binding.rotary(q, k, positions, frequencies, interleaved, sections, magnitude, tensor_layout, False)
+    return _binding.rotary(q, k, positions, frequencies, interleaved, sections, magnitude, tensor_layout)

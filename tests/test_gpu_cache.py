@@ -125,6 +125,18 @@ def test_rotary_gradient(interleaved):
     assert torch.equal(torch.autograd.grad(a.sum(), ql)[0], one)
     b = S.apply_rotary(q.cuda(), kl, pos.cuda(), freq, interleaved)[1]
     _check_rotary(torch.autograd.grad(b.sum(), kl)[0], torch.ones_like(k), -phase, interleaved)
+    # only one of the results is used
+    a, b = S.apply_rotary(ql, kl, pos.cuda(), freq, interleaved)
+    dq, dk = torch.autograd.grad(b.sum(), (ql, kl), allow_unused=True)
+    assert dq is None
+    _check_rotary(dk, torch.ones_like(k), -phase, interleaved)
+    # the gradient of the gradient, in what it was taken along
+    w = gq.cuda().requires_grad_()
+    a = S.apply_rotary(ql, None, pos.cuda(), freq, interleaved)
+    dq, = torch.autograd.grad(a, ql, w, create_graph=True)
+    _check_rotary(torch.autograd.grad(dq, w, q.cuda())[0], q, phase, interleaved)
+    with torch.no_grad():
+        assert not S.apply_rotary(ql, None, pos.cuda(), freq, interleaved).requires_grad
 
 
 # ------------------------------------------------------------------------------------------------------------------- cache
