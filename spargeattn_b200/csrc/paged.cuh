@@ -9,10 +9,12 @@
 
 namespace sparge {
 
-// The border between share c - 1 and share c, for the kernel that joins tiles which lie in several shares.
+// The border in front of a share that begins inside a tile, for the kernel that joins tiles which lie in several shares.
 struct ShareJoin {
-  int pieces;                     // of the tile around the border, in the shares c - 1, c, ...; 0: not the first border in a tile
-  int slot;                       // of the first piece; piece i > 0 has 2 (c - 1 + i)
+  int pieces;                     // of the tile; 0: the share begins with a tile
+  int border;                     // which of the tile's pieces - 1 borders this one is
+  int first;                      // the share of the first piece
+  int slot;                       // of the first piece; piece i > 0 has 2 (first + i)
   int token, row, rows, head;     // the sequence's first row of q; the tile's first row and their count; key head
 };
 
@@ -174,10 +176,9 @@ __device__ __forceinline__ void note_join(const PagedParams& p, long long begin,
   ShareJoin j = {};
   const int c = blockIdx.x;
   if (c < shares && begin > at.first) {
-    const long long before = share_begin(c - 1, units, shares), last = at.first + at.w.blocks(at.tile);
-    if (before <= at.first)
-      j = ShareJoin{share_of(last - 1, units, shares) - (c - 1) + 1, 2 * (c - 1) + (before < at.first), at.token, (int)(at.tile * ROWS),
-                    (int)at.w.tile_rows(at.tile), at.head};
+    const int first = share_of(at.first, units, shares), last = share_of(at.first + at.w.blocks(at.tile) - 1, units, shares);
+    j = ShareJoin{last - first + 1, c - first - 1, first, 2 * first + (share_begin(first, units, shares) < at.first), at.token, (int)(at.tile * ROWS),
+                  (int)at.w.tile_rows(at.tile), at.head};
   }
   p.joins[c] = j;
 }

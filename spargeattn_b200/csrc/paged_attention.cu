@@ -8,42 +8,44 @@
 
 namespace sparge {
 
-// Tiles that lie in several shares: a row of blocks for every border between two shares, most of which find that they have
-// nothing to do. WARPS warps take a row, a piece after the other in turn; the pieces' maxima and sums are read 32 at a time, then
-// their outputs, in an order that does not depend on who was first. Few rows have many pieces (one token over a long
-// context: all 148 shares), so they get four warps each.
-constexpr int kJoinThreads = 256, kJoinBlocks = 8;
+// Tiles that lie in several shares. Every border between two shares has kJoinBlocks blocks; those of all borders inside a tile work on
+// its rows together, so that one token over a long context (36 borders for 16 rows) and a chunk (one border for 256) find the
+// warps that they need: up to eight for a row, which take its pieces in turn. Maxima and sums are read 32 pieces at a time, then
+// the outputs, in an order that does not depend on who was first.
+constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32;
+constexpr int kJoinBlocks = 8;
 
-template <typename T, int D, int WARPS>
+template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(PagedParams p, int rows) {
-  __shared__ float s_part[kJoinThreads / 32][D + 1];
+  __shared__ float s_part[kJoinWarps][D + 1];
   pdl_wait();
-  const int c = blockIdx.x + 1;
-  const ShareJoin a = p.joins[c];
+  const ShareJoin a = p.joins[blockIdx.x + 1];
   if (a.pieces == 0) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp % WARPS, pieces = a.pieces;
-  constexpr int kRows = kJoinThreads / 32 / WARPS;         // of a block at a time
-  for (int r0 = blockIdx.y * kRows; r0 < a.rows; r0 += gridDim.y * kRows) {
-    const int r = min(r0 + warp / WARPS, a.rows - 1);      // (a row twice: the same values)
-    const auto slot = [&](int i) { return (long long)(i == 0 ? a.slot : 2 * (c - 1 + i)) * rows + r; };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, blocks = (a.pieces - 1) * kJoinBlocks;
+  int per_row = 1;                                         // warps
+  while (per_row < kJoinWarps && 2 * per_row * a.rows <= blocks * kJoinWarps) per_row *= 2;
+  const int sub = warp & (per_row - 1), at_once = kJoinWarps / per_row, mine = warp / per_row;
+  for (int r0 = (a.border * kJoinBlocks + blockIdx.y) * at_once; r0 < a.rows; r0 += blocks * at_once) {
+    const int r = min(r0 + mine, a.rows - 1);              // (a row twice: the same values)
+    const auto slot = [&](int i) { return (long long)(i == 0 ? a.slot : 2 * (a.first + i)) * rows + r; };
     float top = -INFINITY;
-    for (int i = lane; i < pieces; i += 32) top = fmaxf(top, p.part_ml[slot(i) * 2]);
+    for (int i = lane; i < a.pieces; i += 32) top = fmaxf(top, p.part_ml[slot(i) * 2]);
     top = warp_max(top);
     float sum = 0.f, acc[D / 32];
 #pragma unroll
     for (int d = 0; d < D / 32; d++) acc[d] = 0.f;
-    for (int i0 = sub; i0 < pieces; i0 += 32 * WARPS) {
-      const int mine = i0 + lane * WARPS;
+    for (int i0 = sub; i0 < a.pieces; i0 += 32 * per_row) {
+      const int own = i0 + lane * per_row;
       float w = 0.f;
-      if (mine < pieces) {
-        w = top == -INFINITY ? 1.f : ex2_approx(p.part_ml[slot(mine) * 2] - top);   // (no key seen: sums of 0, or of NaN)
-        sum += w * p.part_ml[slot(mine) * 2 + 1];
+      if (own < a.pieces) {
+        w = top == -INFINITY ? 1.f : ex2_approx(p.part_ml[slot(own) * 2] - top);   // (no key seen: sums of 0, or of NaN)
+        sum += w * p.part_ml[slot(own) * 2 + 1];
       }
-      const int here = min(32, (pieces - i0 + WARPS - 1) / WARPS);
+      const int here = min(32, (a.pieces - i0 + per_row - 1) / per_row);
 #pragma unroll 8
       for (int i = 0; i < here; i++) {
         const float wi = __shfl_sync(0xffffffffu, w, i);
-        const float* src = p.part_o + slot(i0 + i * WARPS) * D + lane * (D / 32);
+        const float* src = p.part_o + slot(i0 + i * per_row) * D + lane * (D / 32);
         if constexpr (D == 128) {
           const float4 x = *reinterpret_cast<const float4*>(src);
           acc[0] += wi * x.x, acc[1] += wi * x.y, acc[2] += wi * x.z, acc[3] += wi * x.w;
@@ -55,13 +57,13 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(PagedParams p,
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (WARPS > 1) {
+    if (per_row > 1) {
 #pragma unroll
       for (int d = 0; d < D / 32; d++) s_part[warp][lane * (D / 32) + d] = acc[d];
       if (lane == 0) s_part[warp][D] = sum;
       __syncthreads();
       if (sub == 0) {
-        for (int j = 1; j < WARPS; j++) {
+        for (int j = 1; j < per_row; j++) {
 #pragma unroll
           for (int d = 0; d < D / 32; d++) acc[d] += s_part[warp + j][lane * (D / 32) + d];
           sum += s_part[warp + j][D];
@@ -69,7 +71,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(PagedParams p,
       }
       __syncthreads();
     }
-    if (sub == 0 && r0 + warp / WARPS < a.rows) {
+    if (sub == 0 && r0 + mine < a.rows) {
       const float inv = sum != 0.f ? 1.f / sum : 0.f;
       const int seq_row = a.row + r, tok = seq_row / p.group, head = a.head * p.group + seq_row - tok * p.group;
       T* dst = reinterpret_cast<T*>(p.out) + (long long)(a.token + tok) * p.out_token + (long long)head * p.out_head + lane * (D / 32);
@@ -83,9 +85,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(PagedParams p,
 
 template <typename T, int D>
 static cudaError_t join_launch(const PagedParams& p, int rows, cudaStream_t st) {
-  const dim3 grid(p.max_shares - 1, kJoinBlocks);
-  return rows == kDecodeRows ? launch(paged_join_kernel<T, D, 4>, grid, dim3(kJoinThreads), 0, st, true, p, rows)
-                             : launch(paged_join_kernel<T, D, 1>, grid, dim3(kJoinThreads), 0, st, true, p, rows);
+  return launch(paged_join_kernel<T, D>, dim3(p.max_shares - 1, kJoinBlocks), dim3(kJoinThreads), 0, st, true, p, rows);
 }
 
 // 16-bit pages [pages, heads, page_size, D] by their strides; a copy takes up to kBlockKeys rows of one page, `halves` times 64
@@ -101,7 +101,10 @@ static bool page_map(CUtensorMap* m, const void* ptr, const long long* st, const
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Which kernel: tiles of 16 rows or of 256.
+// Which kernel: tiles of 16 rows or of 256. The first reads K and V once for 16 rows and keeps up with HBM; the second's step takes
+// the same time for 1 row and for 128. Measured, us, 16 rows / 256 rows, 32 heads to 4, 16 sequences of 8 000 keys: rows 16: 45 / 62
+// at D = 64, 59 / 74 at D = 128; rows 32: 79 / 57 and 90 / 73; rows 64: 144 / 58 and 181 / 75. One sequence of 30 000 keys, rows 16:
+// 18.6 / 24.4 and 20.8 / 27.9; rows 32: 26.9 / 23.2 and 29.9 / 27.9.
 static int tile_rows(int group, int max_chunk) { return (long long)group * max_chunk <= kDecodeRows ? kDecodeRows : kTileRows; }
 
 static size_t joins_bytes(int shares) { return (sizeof(ShareJoin) * shares + 255) / 256 * 256; }

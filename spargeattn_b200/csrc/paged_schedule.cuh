@@ -94,7 +94,8 @@ SPARGE_SCHED long long share_begin(int c, long long units, int shares) {
 }
 // The share that a unit lies in: the last one that begins at or before it.
 SPARGE_SCHED int share_of(long long unit, long long units, int shares) {
-  return (int)(((unsigned long long)(unit + 1) * shares - 1) / (unsigned long long)units);
+  const unsigned long long x = (unsigned long long)(unit + 1) * shares - 1;
+  return x >> 32 ? (int)(x / (unsigned long long)units) : (int)((unsigned)x / (unsigned)units);
 }
 
 }  // namespace sparge

@@ -148,7 +148,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   int shares;
   Place<kTileRows> at;
   find_share<kTileThreads>(p, s_search, begin, end, units, shares, at);
-  if (tid == 0) note_join(p, begin, units, shares, at);
+  if (tid == kTileThreads - 32) note_join(p, begin, units, shares, at);   // the warp that has nothing else to do
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
