@@ -106,7 +106,6 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     tma_prefetch_desc(&map_v);
   }
   pdl_wait();                                                             // lengths, tables and queries come from the kernels before
-  pdl_trigger();                                                          // the joining kernel's blocks may come and wait
   zero_rest<T, D>(p, blockIdx.x * kDecodeThreads + tid, gridDim.x * kDecodeThreads);
   long long begin, end, units;
   int shares;
@@ -135,22 +134,30 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       u.token = at.token, u.row = (int)(at.tile * R), u.rows = (int)at.w.tile_rows(at.tile), u.head = head;
       u.key = key, u.length = length;
       u.visible0 = p.causal ? length - (int)at.w.tokens : length;
-      if (i >= ST) ok = __all_sync(0xffffffffu, mbar_wait(&bar_empty[slot], ((i / ST) - 1) & 1));
+      // The next unit's place and pages are looked up while a stage becomes free; in front of that, behind the copies.
+      const int now = entry;
+      auto advance = [&]() {
+        fresh = last;
+        if (last) first_piece = false;
+        if (i + 1 < n) {
+          if (!last) at.block++;
+          else next_tile(p, at);
+          entry = entry_at();
+        }
+      };
+      if (i >= ST) {
+        advance();
+        ok = __all_sync(0xffffffffu, mbar_wait(&bar_empty[slot], ((i / ST) - 1) & 1));
+      }
       if (!ok || __any_sync(0xffffffffu, *(volatile int*)&s_fail)) break;
       if (lane == 0) {
         s_unit[slot] = u;
         mbar_arrive_expect_tx(&bar_full[slot], Shape::kStage);
       }
       __syncwarp();
-      load_unit<D>(p, smem + slot * Shape::kStage, &map_k, &map_v, &bar_full[slot], entry, key, length, head, lane);
+      load_unit<D>(p, smem + slot * Shape::kStage, &map_k, &map_v, &bar_full[slot], now, key, length, head, lane);
       issued = i + 1;
-      fresh = last;
-      if (last) first_piece = false;
-      if (i + 1 < n) {
-        if (!last) at.block++;
-        else next_tile(p, at);
-        entry = entry_at();
-      }
+      if (i < ST) advance();
     }
     if (!ok && lane == 0) {
       paged_report(p.dev_status, SPARGE_DEV_TIMEOUT_PRODUCER);

@@ -142,7 +142,6 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     tma_prefetch_desc(&map_v);
   }
   pdl_wait();                                                // lengths, tables and queries come from the kernels before
-  pdl_trigger();                                             // the joining kernel's blocks may come and wait
   zero_rest<T, D>(p, blockIdx.x * kTileThreads + tid, gridDim.x * kTileThreads);
   long long begin, end, units;
   int shares;
@@ -190,14 +189,20 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         }
         for (int j = 0; j < here && ok; j++) {
           const int key = key0 + j * kBlockKeys, i = 2 * (done + j);
-          load(i, &map_k, entry, key, length, head);
-          if (ok) load(i + 1, &map_v, entry, key, length, head);
-          if (j + 1 < here) {
-            entry = entry_at(key + kBlockKeys);
-          } else if (done + here < n) {
-            next_tile(p, at);
-            entry = entry_at(0);
-          }
+          // the next unit's place and pages are looked up while slots become free; behind the first unit's copies
+          const int now = entry;
+          auto advance = [&]() {
+            if (j + 1 < here) {
+              entry = entry_at(key + kBlockKeys);
+            } else if (done + here < n) {
+              next_tile(p, at);
+              entry = entry_at(0);
+            }
+          };
+          if (i > 0) advance();
+          load(i, &map_k, now, key, length, head);
+          if (ok) load(i + 1, &map_v, now, key, length, head);
+          if (i == 0) advance();
         }
         done += here;
         first_piece = false;
