@@ -1,5 +1,6 @@
 /*
- * sparge_b200 -- C ABI of the B200 (sm_100a) block-sparse quantised attention path.
+ * sparge_b200 -- C ABI of the B200 (sm_100a) block-sparse quantised attention path, and (at the end) of the operators beside it:
+ * rotary positions, and a paged key/value cache with the attention over it.
  *
  * Every entry point takes plain device pointers, sizes and a CUDA stream, returns an int status
  * (SPARGE_OK == 0), allocates nothing and keeps no global state unless its comment says so.
@@ -367,6 +368,7 @@ int sparge_paged_attention(const sparge_paged_attention_args* args, sparge_strea
  *
  * pages: `outer` times [num_pages] blocks of page_bytes (a multiple of 16) each: block p of slice o at
  * o * outer_bytes + p * page_stride_bytes. */
+enum { SPARGE_MAX_PAIRS = 65536 }; /* of one call that forks or copies: each is compared with all others */
 size_t sparge_pages_workspace_bytes(int n, int table_width, int num_pages);
 int sparge_allocate_pages(int32_t* page_table, int32_t* seq_lens, int32_t* ref_counts, const int32_t* new_tokens,
                           unsigned char* served, void* workspace, int sequences, int table_width, long long table_stride,

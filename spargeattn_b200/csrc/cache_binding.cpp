@@ -64,6 +64,12 @@ bool rows16(const Tensor& t) {
     if (t.stride(i) % 8 || t.stride(i) < 0) return false;
   return true;
 }
+// Whether no two elements share a place, as far as single strides tell.
+bool apart(const Tensor& t) {
+  for (int64_t i = 0; i < t.dim(); i++)
+    if (t.size(i) > 1 && t.stride(i) == 0) return false;
+  return true;
+}
 const int32_t* int32s(const Tensor& t, int64_t n, const char* name) {
   NEED(t.scalar_type() == at::kInt && t.dim() == 1 && t.is_contiguous(), name, " must be a contiguous int32 vector");
   if (n >= 0) NEED(t.numel() == n, name, " must have ", n, " elements, has ", t.numel());
@@ -280,7 +286,7 @@ CacheTensors cache_of(PyObject* const* args, int64_t tokens, at::ScalarType type
   const int64_t ps = kp.size(2);
   NEED(ps >= 16 && ps <= 256 && (ps & (ps - 1)) == 0, "page_size must be a power of two from 16 to 256, is ", ps);
   NEED(kp.size(0) < (1 << 29) && kp.size(1) >= 1 && kp.size(1) <= INT_MAX, "k_pages has too many pages, or no heads");
-  for (const Tensor* p : {&kp, &vp}) NEED(p->stride(3) == 1 && rows16(*p), "the pages' rows must be dense and 16-byte aligned");
+  for (const Tensor* p : {&kp, &vp}) NEED(p->stride(3) == 1 && rows16(*p) && apart(*p), "the pages' rows must be dense, 16-byte aligned and apart");
   NEED(t.table->scalar_type() == at::kInt && t.table->dim() == 2, "page_table must be int32 [sequences, pages of a sequence]");
   const int64_t S = t.table->size(0), W = t.table->size(1);
   NEED(W <= 1 || t.table->stride(1) == 1, "page_table's rows must be dense");
@@ -373,7 +379,7 @@ PyObject* attention_impl(PyObject* const* args, Py_ssize_t nargs) {
   const Tensor* out_given = given ? &tensor(args[9], "out") : nullptr;
   if (given) {
     NEED(out_given->sizes() == q.sizes() && out_given->scalar_type() == q.scalar_type(), "out must have q's shape and type");
-    NEED(out_given->stride(2) == 1 && rows16(*out_given), "out's rows must be dense and 16-byte aligned");
+    NEED(out_given->stride(2) == 1 && rows16(*out_given) && apart(*out_given), "out's rows must be dense, 16-byte aligned and apart");
   }
   const c10::Device dev = q.device();
   on_gpu(q, dev, "q");
@@ -510,7 +516,7 @@ PyObject* fork_impl(PyObject* const* args, Py_ssize_t nargs) {
   NEED(p.page_size >= 16 && p.page_size <= 256 && (p.page_size & (p.page_size - 1)) == 0, "page_size must be a power of two from 16 to 256, is ", p.page_size);
   const Tensor &src = tensor(args[4], "src"), &dst = tensor(args[5], "dst");
   int32s(src, -1, "src"), int32s(dst, src.numel(), "dst");
-  NEED(src.numel() <= (1 << 20), "too many forks in one call");
+  NEED(src.numel() <= SPARGE_MAX_PAIRS, "at most ", SPARGE_MAX_PAIRS, " forks in one call");
   const int n = (int)src.numel();
   const c10::Device dev = p.t->device();
   on_gpu(*p.t, dev, "pages"), table_on_gpu(t, dev), on_gpu(src, dev, "src"), on_gpu(dst, dev, "dst");
@@ -545,7 +551,7 @@ PyObject* copy_impl(PyObject* const* args, Py_ssize_t nargs) {
   const PoolArgs p = pool_of(args[0]);
   const Tensor &src = tensor(args[1], "src"), &dst = tensor(args[2], "dst");
   int32s(src, -1, "src"), int32s(dst, src.numel(), "dst");
-  NEED(src.numel() <= (1 << 20), "too many pages in one call");
+  NEED(src.numel() <= SPARGE_MAX_PAIRS, "at most ", SPARGE_MAX_PAIRS, " pages in one call");
   NEED(p.pages < (1 << 29), "too many pages");
   const c10::Device dev = p.t->device();
   on_gpu(*p.t, dev, "pages"), on_gpu(src, dev, "src"), on_gpu(dst, dev, "dst");

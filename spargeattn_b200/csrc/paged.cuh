@@ -202,8 +202,8 @@ __device__ __forceinline__ void zero_rest(const PagedParams& p, int thread, int 
 // 128-byte swizzle). Keys that the sequence does not have, and pages that the pool does not have, are read at a page number
 // behind the last one, where the copy engine fills in zeros. So every tile is complete, and nothing of what an earlier owner left
 // behind is in it but the rest of the one page that the length ends in.
-// A lane's entry of the table for a unit (the pages of its pieces, lane by lane), read while the unit before it is under way: a look
-// into the table just before each copy made the copies the slowest part of the kernel over long chunks (3 750 cycles a unit).
+// A lane's entry of the table for a unit (the pages of its pieces, lane by lane), read while the unit before it is under way (just
+// before the copies: 216 us for 64 sequences of up to 8 191 keys in pages of 16, where this takes 200).
 __device__ __forceinline__ int table_entry(const PagedParams& p, int seq, int key, int length) {
   return key < length ? p.table[seq * p.table_stride + (key >> p.page_shift)] : 0;
 }

@@ -402,6 +402,7 @@ extern "C" int sparge_fork_sequences(void* pages, long long outer, long long out
   const PageTable t{page_table, seq_lens, ref_counts, table_stride, sequences, table_width, num_pages, page_size};
   const PagePool pool{(char*)pages, outer, outer_bytes, page_stride_bytes, page_bytes};
   if (!table_ok(t) || !pool_ok(pool) || n < 0) return SPARGE_ERR_INVALID_ARG;
+  if (n > SPARGE_MAX_PAIRS) return SPARGE_ERR_TOO_LARGE;
   if (n == 0) return SPARGE_OK;
   if ((sequences && ((table_width && !page_table) || !seq_lens)) || (num_pages && (!ref_counts || !pages)) || !src || !dst || !served || !workspace)
     return SPARGE_ERR_NULL;
@@ -443,6 +444,7 @@ extern "C" int sparge_copy_pages(void* pages, long long outer, long long outer_b
   using namespace sparge;
   const PagePool pool{(char*)pages, outer, outer_bytes, page_stride_bytes, page_bytes};
   if (!pool_ok(pool) || n < 0 || num_pages < 0) return SPARGE_ERR_INVALID_ARG;
+  if (n > SPARGE_MAX_PAIRS) return SPARGE_ERR_TOO_LARGE;
   if (n == 0 || outer == 0 || page_bytes == 0) return SPARGE_OK;
   if ((num_pages && !pages) || !src || !dst) return SPARGE_ERR_NULL;
   // one pair at a time fills the GPU only where pages are large or the pool has many slices

@@ -16,6 +16,7 @@ cu_seqlens are read when the kernels run, so a captured step follows them from r
 
 Arguments that do not fit are ValueError, CPU tensors RuntimeError. What only the device can see (a page number outside the
 pool, a length outside the table) is skipped without touching other memory and reported through `ops.check_device_status()`.
+Nothing here has a gradient. The first call on a device should precede graph capture: it sets up the word that reports go to.
 """
 import torch
 
@@ -88,8 +89,9 @@ def fork_sequences(pages, page_table, seq_lens, ref_counts, src, dst):
 
 @_skip_frame
 def compact_pages(pages, page_table, ref_counts):
-    """Moves the pages in use to the front of the pool, in every layer that `pages` holds, and rewrites table and counts in place.
-    Returns their number, int32 [1] on the device: pages from there on are free."""
+    """Moves the pages in use (a count above 0) to the front of the pool, in every layer that `pages` holds, and rewrites table and
+    counts in place. Returns their number, int32 [1] on the device: pages from there on are free. A page that the program holds by
+    a count of its own, without an entry of the table, moves like the others."""
     return _binding.compact_pages(pages, page_table, ref_counts)
 
 

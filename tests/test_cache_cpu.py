@@ -60,7 +60,8 @@ def test_cpu_tensors_are_refused():
     (dict(k_pages=torch.zeros(9, 2, 16, 64, dtype=BF)), "same shape"), (dict(seq_lens=torch.ones(3, dtype=torch.int32)), "seq_lens"),
     (dict(seq_lens=torch.ones(2, dtype=torch.int64)), "int32"), (dict(page_table=torch.zeros(2, 4, dtype=torch.int64)), "int32"),
     (dict(cu_seqlens=torch.zeros(2, dtype=torch.int32)), "cu_seqlens"), (dict(max_chunk=-1), "max_chunk"), (dict(scale=math.nan), "scale"),
-    (dict(out=torch.zeros(2, 4, 64)), "out"), (dict(q=torch.zeros(2, 4, 65, dtype=BF)[..., 1:]), "aligned"),
+    (dict(out=torch.zeros(2, 4, 64)), "out"), (dict(out=torch.zeros(2, 1, 64, dtype=BF).expand(2, 4, 64)), "apart"),
+    (dict(k_pages=torch.zeros(1, 2, 16, 64, dtype=BF).expand(8, 2, 16, 64)), "apart"), (dict(q=torch.zeros(2, 4, 65, dtype=BF)[..., 1:]), "aligned"),
     (dict(k_pages=torch.zeros(8, 2, 16, 96, dtype=BF), v_pages=torch.zeros(8, 2, 16, 96, dtype=BF)), "headdim"),
     (dict(k_pages=torch.zeros(0, 2, 16, 64, dtype=BF), v_pages=torch.zeros(0, 2, 16, 64, dtype=BF)), "no pages")])
 def test_attention_refuses(change, text):
@@ -86,6 +87,8 @@ def test_bookkeeping_refuses():
                        (lambda: S.free_sequences(table, lens, refs.long(), one), "ref_counts"), (lambda: S.free_sequences(table, lens, refs, one.long()), "sequences"),
                        (lambda: S.fork_sequences(pool[:, :7], table, lens, refs, one, one), "each of the 7"), (lambda: S.fork_sequences(pool, table, lens, refs, one, lens), "dst"),
                        (lambda: S.compact_pages(pool.transpose(2, 3), table, refs), "one block"), (lambda: S.copy_pages(pool, one, lens), "dst"),
+                       (lambda: S.copy_pages(pool, torch.zeros(65537, dtype=torch.int32), torch.zeros(65537, dtype=torch.int32)), "at most 65536"),
+                       (lambda: S.fork_sequences(pool, table, lens, refs, torch.zeros(65537, dtype=torch.int32), torch.zeros(65537, dtype=torch.int32)), "at most"),
                        (lambda: S.copy_pages(pool[0, 0], one, one), "pages"), (lambda: S.copy_pages(pool[:, :, :, ::2], one, one), "one block")):
         with pytest.raises(ValueError, match=text):
             call()
@@ -104,6 +107,7 @@ def test_c_entries_check_their_arguments():
     assert L.sparge_allocate_pages(one, one, one, one, one, one, 2, -1, 4, 8, 16, None) == _cabi.ERR_INVALID_ARG
     assert L.sparge_free_sequences(one, one, one, None, 1, 2, 4, 4, 8, None, None) == _cabi.ERR_NULL
     assert L.sparge_copy_pages(one, 1, 0, 64, 24, one, one, 1, 8, None, None) == _cabi.ERR_INVALID_ARG      # pages of 24 bytes
+    assert L.sparge_copy_pages(one, 1, 0, 64, 32, one, one, 65537, 8, None, None) == _cabi.ERR_TOO_LARGE
     assert L.sparge_copy_pages(None, 1, 0, 64, 32, one, one, 1, 8, None, None) == _cabi.ERR_NULL
     assert L.sparge_compact_pages(one, 1, 0, 32, 32, one, one, None, one, 1, 4, 4, 8, None) == _cabi.ERR_NULL
     assert L.sparge_fork_sequences(one, 1, 0, 32, 32, one, one, one, one, None, one, one, 1, 2, 4, 4, 8, 16, None, None) == _cabi.ERR_NULL
