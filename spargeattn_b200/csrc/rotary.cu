@@ -14,7 +14,7 @@
 namespace sparge {
 
 constexpr int kRotThreads = 256;
-constexpr int kRotTokens = 8;      // most tokens of a block
+constexpr int kRotTokens = 8;      // most tokens of a block: a power of two
 
 // What keeps HBM busy is blocks: six of them where the compiler needs no more registers than that (neighbouring pairs: 157 us for
 // the forward and backward pass of [1,12,32760,128] queries and keys, 174 with four), four where a unit has two halves (partial
@@ -42,7 +42,7 @@ struct RotParams {
   long long pos_st[3];
   const double* freq;
   float magnitude;
-  int tokens_per_block;
+  int tokens_per_block, tok_shift;   // a power of two
   // append
   const int32_t *table, *seq_lens, *cu;
   long long table_stride;
@@ -84,6 +84,23 @@ __device__ __forceinline__ void raw_store(T* p, const Raw<T, V>& r) {
   }
 }
 
+// The batch that a token lies in. A division of 64 bits is as many instructions as turning two heads.
+__device__ __forceinline__ int batch_of(const RotParams& p, long long t) {
+  if (p.B == 1) return 0;
+  return t >> 32 ? (int)(t / p.N) : (int)((unsigned)t / (unsigned)p.N);
+}
+
+// Two neighbours rounded by one instruction where there is one.
+__device__ __forceinline__ void round_two(float& x, float& y, float u, float w) { x = u, y = w; }
+__device__ __forceinline__ void round_two(__half& x, __half& y, float u, float w) {
+  const __half2 h = __floats2half2_rn(u, w);
+  x = h.x, y = h.y;
+}
+__device__ __forceinline__ void round_two(__nv_bfloat16& x, __nv_bfloat16& y, float u, float w) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(u, w);
+  x = h.x, y = h.y;
+}
+
 template <>
 struct Elem<float> {
   static __device__ __forceinline__ float to_float(float v) { return v; }
@@ -117,13 +134,24 @@ struct HeadBatch {
     for (int j = 0; j < kAhead; j++) {
       if (j >= left) break;
       if (ROT && turn) {
+        float u[kPairs], w[kPairs];
 #pragma unroll
         for (int i = 0; i < kPairs; i++) {
-          T& lo = INTER ? a[j].v[2 * i] : a[j].v[i];
-          T& hi = INTER ? a[j].v[2 * i + 1] : b[j].v[i];
-          const float u = Elem<T>::to_float(lo), w = Elem<T>::to_float(hi);
-          lo = Elem<T>::from_float(u * c[i].x - w * c[i].y);
-          hi = Elem<T>::from_float(u * c[i].y + w * c[i].x);
+          const float x = Elem<T>::to_float(INTER ? a[j].v[2 * i] : a[j].v[i]), z = Elem<T>::to_float(INTER ? a[j].v[2 * i + 1] : b[j].v[i]);
+          u[i] = x * c[i].x - z * c[i].y;
+          w[i] = x * c[i].y + z * c[i].x;
+        }
+        if constexpr (INTER) {
+#pragma unroll
+          for (int i = 0; i < kPairs; i++) round_two(a[j].v[2 * i], a[j].v[2 * i + 1], u[i], w[i]);
+        } else if constexpr (kPairs % 2 == 0) {
+#pragma unroll
+          for (int i = 0; i < kPairs; i += 2) {
+            round_two(a[j].v[i], a[j].v[i + 1], u[i], u[i + 1]);
+            round_two(b[j].v[i], b[j].v[i + 1], w[i], w[i + 1]);
+          }
+        } else {
+          a[j].v[0] = Elem<T>::from_float(u[0]), b[j].v[0] = Elem<T>::from_float(w[0]);
         }
         if (!INTER) raw_store<T, V, VEC>(y + pairs, b[j]);
       }
@@ -148,7 +176,7 @@ __device__ __forceinline__ RotShare rot_share(const RotParams& p, const RotSlot&
   s.per = min(s.units, kRotThreads);
   const int groups = kRotThreads / s.per;
   s.group = tid / s.per, s.unit = tid - s.group * s.per;
-  s.step = max(1, groups / p.tokens_per_block);
+  s.step = max(1, groups >> p.tok_shift);
   s.in = s.group < groups;
   return s;
 }
@@ -211,10 +239,10 @@ __global__ void __launch_bounds__(kRotThreads, (RotShape<INTER, ROT>::kBlocks)) 
   if (!PAGED) {
     const RotSlot& sl = p.slot[0];
     const RotShare s = rot_share<V, INTER, ROT>(p, sl, tid);
-    const int tok = s.group % TOK, h0 = s.group / TOK;
+    const int tok = s.group & (TOK - 1), h0 = s.group >> p.tok_shift;
     const long long t = t0 + tok;
     if (s.in && s.group < TOK * s.step && t < tokens && h0 < sl.heads) {
-      const int b = (int)(t / p.N);
+      const int b = batch_of(p, t);
       const bool turn = s.unit < s.rot_units;
       batch.load(reinterpret_cast<const T*>(sl.x) + b * sl.xb + (t - (long long)b * p.N) * sl.xn + h0 * sl.xh + s.channel(s.unit, V), s.step * sl.xh,
                  (sl.heads - h0 + s.step - 1) / s.step, s.pairs, turn, false);
@@ -232,7 +260,7 @@ __global__ void __launch_bounds__(kRotThreads, (RotShape<INTER, ROT>::kBlocks)) 
     } else {
       int axis = 0;
       for (int first = 0; axis + 1 < p.axes && pair >= first + p.sections[axis]; axis++) first += p.sections[axis];
-      const int b = (int)(t / p.N);
+      const int b = batch_of(p, t);
       const long long at = axis * p.pos_st[0] + b * p.pos_st[1] + (t - (long long)b * p.N) * p.pos_st[2];
       pos = p.pos64 ? (double)reinterpret_cast<const long long*>(p.positions)[at]
                     : (double)reinterpret_cast<const int32_t*>(p.positions)[at];
@@ -250,10 +278,10 @@ __global__ void __launch_bounds__(kRotThreads, (RotShape<INTER, ROT>::kBlocks)) 
     const RotShare s = rot_share<V, INTER, ROT>(p, sl, tid);
     const int groups = kRotThreads / s.per;
     for (int g = s.group; g < TOK * s.step && s.in; g += groups) {
-      const int tok = g % TOK, h0 = g / TOK;
+      const int tok = g & (TOK - 1), h0 = g >> p.tok_shift;
       const long long t = t0 + tok;
       if (t >= tokens) continue;
-      const int b = PAGED ? 0 : (int)(t / p.N);
+      const int b = PAGED ? 0 : batch_of(p, t);
       const T* x = reinterpret_cast<const T*>(sl.x) + b * sl.xb + (t - (long long)b * p.N) * sl.xn;
       T* y = reinterpret_cast<T*>(sl.y);
       bool zero = false;
@@ -289,7 +317,8 @@ template <typename T, bool INTER, bool PAGED, bool ROT>
 static int rotary_launch(RotParams& p, bool vec, cudaStream_t st) {
   const long long tokens = (long long)p.B * p.N;
   // Few tokens: a block each, so that a step's heads spread over the GPU; many: eight, whose angles share one pass.
-  p.tokens_per_block = tokens >= 8 * 148 ? kRotTokens : tokens >= 2 * 148 ? 2 : 1;
+  p.tok_shift = tokens >= 8 * 148 ? 3 : tokens >= 2 * 148 ? 1 : 0;
+  p.tokens_per_block = 1 << p.tok_shift;
   const size_t smem = sizeof(float2) * p.tokens_per_block * p.pairs;
   const long long blocks = (tokens + p.tokens_per_block - 1) / p.tokens_per_block;
   if (blocks > 0x7fffffffLL) return SPARGE_ERR_TOO_LARGE;
