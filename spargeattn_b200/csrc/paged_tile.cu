@@ -7,9 +7,11 @@
 // A CTA has two tiles of 128 rows (the rows of one key head: tokens by query heads of its group, so grouped heads share every
 // key that is fetched) and works on both in turn: while the softmax warps of one are busy, the tensor cores do P V and the next
 // Q K^T of the other. Their S, P and O fill tensor memory: columns [0, 128) S and P of the first, [128, 256) of the second,
-// [256, 384) and [384, 512) their outputs. 12 warps: 0-3 and 4-7 softmax and epilogue of a tile each, 8 the copies, 9 and
-// 10 the products of a tile each (11 completes a warpgroup, whose registers the softmax warps take over). One CTA on each SM takes an equal run of the call's units (paged_schedule.cuh); the copies run ahead over the borders
-// of tiles, heads and sequences, and a tile's queries are fetched while the last product of the tile before it is under way.
+// [256, 384) and [384, 512) their outputs. 12 warps: 0-3 and 4-7 softmax and epilogue of a tile each, 8 the copies, 9 the
+// products (10 and 11 complete a warpgroup, whose registers the softmax warps take over). One warp asks for the products of both
+// tiles, in turn: with a warp for each they fall into step and want the exponential unit at the same time (1 273 us against 1 176).
+// One CTA on each SM takes an equal run of the call's units (paged_schedule.cuh); the copies run ahead over the borders of tiles,
+// heads and sequences, and a tile's queries are fetched while the last product of the tile before it is under way.
 //
 // The products of a step of 128 keys take 2 048 cycles for the two tiles at D = 128 and the exponentials as many (16 a cycle on
 // an SM), so both would have to run all the time; measured: 3 300 cycles a step, tensor cores 63 % and the exponential unit 65 %

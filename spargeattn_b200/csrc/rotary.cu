@@ -16,10 +16,11 @@ namespace sparge {
 constexpr int kRotThreads = 256;
 constexpr int kRotTokens = 8;      // most tokens of a block: a power of two
 
-// What keeps HBM busy is blocks: six of them where the compiler needs no more registers than that (neighbouring pairs: 157 us for
-// the forward and backward pass of [1,12,32760,128] queries and keys, 174 with four), four where a unit has two halves (partial
-// rotation of [4097, 16 + 4, 128]: 12.1 us, 25.5 with six, which spill). Heads loaded together: more in flight and more registers
-// each (two against four: 157 and 183 us); without a rotation there is nothing else to hold, and four.
+// What keeps HBM busy is blocks on an SM, and heads loaded together; both take registers. Forward and backward pass of
+// [1,12,32760,128] queries and keys, neighbouring pairs: six blocks of two heads 144 us, five 151, seven 160 (they spill), four of
+// four heads 153, eight of one 164. A unit of two halves needs more: partial rotation of [4097, 16 + 4, 128] with four blocks 10.0
+// us, five 14.1, six 25.7. Without a rotation there is nothing else to hold: four heads (17.0 us for 9 450 tokens' keys and values,
+// two 19.1). Tokens of a block: eight 144 us, four 176, sixteen 150.
 template <bool INTER, bool ROT>
 struct RotShape {
   static constexpr int kAhead = ROT ? 2 : 4, kBlocks = ROT && INTER ? 6 : 4;
