@@ -61,9 +61,11 @@ void on_gpu(const Tensor& t, c10::Device dev, const char* name) {
 bool rows16(const Tensor& t) {
   if (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16) return false;
   for (int64_t i = 0; i + 1 < t.dim(); i++)
-    if (t.stride(i) % 8 || t.stride(i) < 0) return false;
+    if (t.size(i) > 1 && (t.stride(i) % 8 || t.stride(i) < 0)) return false;
   return true;
 }
+// The stride of a dimension; of one without neighbours, where a view may say anything, one that fits.
+long long stride_of(const Tensor& t, int i) { return t.size(i) > 1 ? t.stride(i) : t.size(-1); }
 // Whether no two elements share a place, as far as single strides tell.
 bool apart(const Tensor& t) {
   for (int64_t i = 0; i < t.dim(); i++)
@@ -296,7 +298,7 @@ CacheTensors cache_of(PyObject* const* args, int64_t tokens, at::ScalarType type
   else NEED(tokens == S, "without cu_seqlens every sequence has one token: got ", tokens, " tokens for ", S, " sequences");
   NEED(tokens <= INT_MAX, "too many tokens");
   c.k_pages = kp.data_ptr(), c.v_pages = vp.data_ptr(), c.page_table = t.table->data_ptr<int32_t>();
-  for (int i = 0; i < 3; i++) c.k_st[i] = kp.stride(i), c.v_st[i] = vp.stride(i);
+  for (int i = 0; i < 3; i++) c.k_st[i] = stride_of(kp, i), c.v_st[i] = stride_of(vp, i);
   c.table_stride = t.table->stride(0);
   c.sequences = (int)S, c.table_width = (int)W, c.num_pages = (int)kp.size(0), c.page_size = (int)ps, c.kv_heads = (int)kp.size(1);
   c.D = (int)kp.size(3), c.tokens = (int)tokens;
@@ -398,7 +400,7 @@ PyObject* attention_impl(PyObject* const* args, Py_ssize_t nargs) {
   const c10::DataPtr ws = scratch(a.workspace_bytes);
   a.workspace = ws.get();
   a.q = q.data_ptr(), a.out = out.data_ptr();
-  a.q_st[0] = q.stride(0), a.q_st[1] = q.stride(1), a.out_st[0] = out.stride(0), a.out_st[1] = out.stride(1);
+  a.q_st[0] = stride_of(q, 0), a.q_st[1] = stride_of(q, 1), a.out_st[0] = stride_of(out, 0), a.out_st[1] = stride_of(out, 1);
   a.dev_status = status_of(dev);
   check(sparge_paged_attention(&a, stream_of(dev)), "paged_attention");
   return want_lse ? pair(out, lse) : THPVariable_Wrap(out);

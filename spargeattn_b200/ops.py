@@ -93,7 +93,7 @@ def check_device_status(device=None) -> int:
     if code == 5:
         raise RuntimeError("device status 5: copy_pages was given a destination twice, or one that is a source too")
     if code != 0:
-        raise RuntimeError(f"sparge_attn_fwd reported device status {code} (a bounded wait expired)")
+        raise RuntimeError(f"an attention kernel reported device status {code} (a bounded wait expired)")
     return code
 
 

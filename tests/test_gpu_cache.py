@@ -251,6 +251,21 @@ def test_chunks_of_many_heads(ps, D, dtype, Hq, Hkv):
         _check_attention(out, lse, q, c, lengths, [0, 3, 20], causal)
 
 
+def test_dimensions_of_one_have_no_stride():
+    """What a view says about a dimension of size one is not looked at."""
+    c = _make([100], 1, 64, 16, BF, 22, spare=0)
+    q = torch.randn(1, 4, 64, generator=_gen(22)).to(BF).cuda()
+    want = S.paged_attention(q, **c)
+    P = c["k_pages"].shape[0]
+    for n in ("k_pages", "v_pages"):
+        c[n] = c[n].as_strided((P, 1, 16, 64), (16 * 64, 3, 64, 1))
+    out = torch.zeros(300, dtype=BF, device="cuda")[:256].as_strided((1, 4, 64), (5, 64, 1))
+    assert torch.equal(S.paged_attention(q.as_strided((1, 4, 64), (7, 64, 1)), **c, out=out), want)
+    k = torch.randn(1, 1, 64, generator=_gen(23)).to(BF).cuda()
+    S.append_kv(k.as_strided((1, 1, 64), (1, 1, 1)), k, **c)
+    assert torch.equal(c["k_pages"][c["page_table"][0, 6], :, 3], k[0])
+
+
 def test_output_over_the_queries():
     """Every row of q is read before its output is written: out may be q itself."""
     for chunk, length in ((1, 5000), (300, 2000)):
