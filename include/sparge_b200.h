@@ -327,10 +327,10 @@ int sparge_append_kv(const sparge_append_args* args, sparge_stream_t stream);
  * own position, seq_lens - n + j; else all of the sequence's. A row that sees no key gives zeros and an lse of -inf.
  * q, out [tokens, q_heads, D] with strides {token, head}, 16-byte aligned rows; D 64 or 128; lse [tokens, q_heads]
  * contiguous, or NULL. max_chunk: an upper bound of the new tokens of one sequence; it chooses the kernel, results hold
- * whatever it says. Rows of no sequence: zeros (lse -inf) with zero_rest, else left as they were. Scores, sums and products are
- * accumulated in 32 bits; probabilities are rounded to the 16-bit type before the product with V. Keys at or behind the
- * length are never read into a result, whatever their pages hold. A page number outside the pool, or a length outside the
- * table, is reported as SPARGE_DEV_BAD_PAGE and the rows of that sequence are undefined.
+ * whatever it says. Rows of no sequence: left as they were with zero_rest 0, zeros in out and -inf in lse with 1, -inf in lse
+ * alone with 2. Scores, sums and products are accumulated in 32 bits; probabilities are rounded to the 16-bit type before the
+ * product with V. Keys at or behind the length are never read into a result, whatever their pages hold. A page number outside
+ * the pool, or a length outside the table, is reported as SPARGE_DEV_BAD_PAGE and the rows of that sequence are undefined.
  * workspace: sparge_paged_attention_workspace_bytes() bytes of device memory, 16-byte aligned, of this call alone. */
 typedef struct {
   sparge_cache cache;

@@ -395,7 +395,7 @@ PyObject* attention_impl(PyObject* const* args, Py_ssize_t nargs) {
     lse = fresh({q.size(0), q.size(1)}, at::kFloat, dev);
     a.lse = lse.data_ptr<float>();
   }
-  a.zero_rest = !given;
+  a.zero_rest = given ? 2 : 1;                             // a given out keeps its rows of no sequence; the lse is the call's own
   a.workspace_bytes = sparge_paged_attention_workspace_bytes(a.q_heads, c.kv_heads, c.D, a.max_chunk);
   const c10::DataPtr ws = scratch(a.workspace_bytes);
   a.workspace = ws.get();

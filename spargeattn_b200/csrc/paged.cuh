@@ -25,7 +25,7 @@ struct PagedParams {
   long long q_token, q_head, out_token, out_head, table_stride;
   const int32_t *cu, *seq_lens, *table;
   int tokens, sequences, width, num_pages, page_size, page_shift, kv_heads, group;
-  bool causal, zero_rest;
+  bool causal, zero_out, zero_lse;
   float scale_log2;
   ShareJoin* joins;               // [max_shares]
   float* part_o;                  // [shares][2][rows][D]: the share's first tile, its last one
@@ -183,18 +183,18 @@ __device__ __forceinline__ void note_join(const PagedParams& p, long long begin,
   p.joins[c] = j;
 }
 
-// Rows of q that belong to no sequence become zeros.
+// Rows of q that belong to no sequence become zeros, and minus infinity in lse.
 template <typename T, int D>
 __device__ __forceinline__ void zero_rest(const PagedParams& p, int thread, int threads) {
-  if (!p.zero_rest || !p.cu) return;
+  if (!p.cu || !(p.zero_out || p.zero_lse)) return;
   const int lo = max(0, min(p.cu[0], p.tokens)), hi = max(lo, min(p.cu[p.sequences], p.tokens)), heads = p.kv_heads * p.group;
   const long long rows = (long long)(p.tokens - (hi - lo)) * heads;
   constexpr int kWords = D * (int)sizeof(T) / 16;
   for (long long i = thread; i < rows * kWords; i += threads) {
     const long long r = i / kWords, t = r / heads, token = t < lo ? t : t - lo + hi;
     const int h = (int)(r - t * heads), word = (int)(i - r * kWords);
-    reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + token * p.out_token + h * p.out_head)[word] = make_uint4(0, 0, 0, 0);
-    if (word == 0 && p.lse) p.lse[token * heads + h] = -INFINITY;
+    if (p.zero_out) reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + token * p.out_token + h * p.out_head)[word] = make_uint4(0, 0, 0, 0);
+    if (word == 0 && p.zero_lse) p.lse[token * heads + h] = -INFINITY;
   }
 }
 

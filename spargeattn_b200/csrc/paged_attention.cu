@@ -147,7 +147,7 @@ extern "C" int sparge_paged_attention(const sparge_paged_attention_args* a, spar
   p.cu = c.cu_seqlens, p.seq_lens = c.seq_lens, p.table = c.page_table;
   p.tokens = c.tokens, p.sequences = c.sequences, p.width = c.table_width, p.num_pages = c.num_pages, p.page_size = c.page_size;
   while ((1 << p.page_shift) < c.page_size) p.page_shift++;
-  p.kv_heads = c.kv_heads, p.group = group, p.causal = a->is_causal != 0, p.zero_rest = a->zero_rest != 0;
+  p.kv_heads = c.kv_heads, p.group = group, p.causal = a->is_causal != 0, p.zero_out = a->zero_rest && a->zero_rest != 2, p.zero_lse = a->lse && a->zero_rest;
   p.scale_log2 = a->scale * 1.4426950408889634f;
   p.joins = reinterpret_cast<ShareJoin*>(a->workspace);
   p.part_o = reinterpret_cast<float*>(reinterpret_cast<char*>(a->workspace) + joins_bytes(p.max_shares));

@@ -54,8 +54,8 @@ def paged_attention(q, k_pages, v_pages, page_table, seq_lens, cu_seqlens=None, 
     seq_len - n + j (`is_causal=False`: all of the sequence's). A row that sees no key gives zeros and an lse of -inf. D is 64
     or 128, scale defaults to D ** -0.5. `max_chunk`, an upper bound of the new tokens of one sequence, chooses the kernel
     (without it: all tokens, or 1 without cu_seqlens); results hold whatever it says. Rows of no sequence are zeros, or left as
-    they were in a given `out`. What pages hold behind the length never reaches a result; an infinity or NaN in V at a
-    position that a row does not see but a later row of its chunk does may (0 * inf), as it does in a masked product."""
+    they were in a given `out`; their lse is -inf. What pages hold behind the length never reaches a result; an infinity or NaN
+    in V at a position that a row does not see but a later row of its chunk does may (0 * inf), as it does in a masked product."""
     _status(q)
     return _binding.paged_attention(q, k_pages, v_pages, page_table, seq_lens, cu_seqlens, max_chunk, is_causal, scale, out, return_lse)
 

@@ -754,3 +754,28 @@ def test_streams_and_threads():
     for t in threads:
         t.join()
     assert not wrong
+
+
+@pytest.mark.parametrize("chunk", [1, 200])
+def test_lse_of_rows_of_no_sequence_beside_a_given_out(chunk):
+    """The lse is the call's own tensor: rows of no sequence are -inf there, also where a given out keeps what it had."""
+    H, D = 4, 64
+    lengths, chunks = [300, 250], [chunk, chunk]
+    c = _make(lengths, 2, D, 16, BF, 24)
+    cu = _cu(chunks, start=3)
+    T = cu[-1] + 5
+    q = torch.randn(T, H, D, generator=_gen(24)).to(BF).cuda()
+    cut = torch.tensor(cu, dtype=torch.int32).cuda()
+    want, want_lse = S.paged_attention(q, **c, cu_seqlens=cut, max_chunk=chunk, return_lse=True)
+    out = torch.full_like(q, 7.0)
+    stale = torch.full((T, H), 7.0, device="cuda")                     # what the call's own tensor may find in its memory
+    del stale
+    _, lse = S.paged_attention(q, **c, cu_seqlens=cut, max_chunk=chunk, out=out, return_lse=True)
+    assert torch.equal(lse, want_lse) and (lse[:3] == -math.inf).all() and (lse[cu[-1]:] == -math.inf).all()
+    assert torch.equal(out[3: cu[-1]], want[3: cu[-1]]) and (out[:3] == 7).all() and (out[cu[-1]:] == 7).all()
+    # no sequence at all
+    none = dict(c, page_table=c["page_table"][:0], seq_lens=c["seq_lens"][:0], cu_seqlens=_i32(0), max_chunk=chunk)
+    out, lse = S.paged_attention(q, **none, out=torch.full_like(q, 7.0), return_lse=True)
+    assert (out == 7).all() and (lse == -math.inf).all()
+    out, lse = S.paged_attention(q, **none, return_lse=True)
+    assert (out == 0).all() and (lse == -math.inf).all()
