@@ -441,7 +441,9 @@ int page_size_of(PyObject* o) {
   return (int)ps;
 }
 
-// Pages [..., pages, kv_heads, page_size, head_dim], each page one block of memory, the dimensions in front one stride.
+// Pages [..., pages, kv_heads, page_size, head_dim], each page one block of memory, the dimensions in front one stride. Inside a page
+// the heads come first, or the tokens: then the two dimensions are seen through a transpose, and the page has to have a size that the
+// cache knows (what looks like it with another size is not a cache's).
 struct PoolArgs {
   const Tensor* t;
   long long outer, outer_bytes, stride_bytes, page_bytes;
@@ -456,10 +458,13 @@ PoolArgs pool_of(PyObject* o) {
   const int e = (int)t.element_size();
   NEED(t.numel() > 0, "pages must not be empty");
   p.pages = t.size(dim - 4), p.page_size = t.size(dim - 2);
-  NEED(t.stride(dim - 1) == 1 && t.stride(dim - 2) == t.size(dim - 1) && t.stride(dim - 3) == t.size(dim - 1) * t.size(dim - 2),
-       "a page must be one block of memory");
-  p.page_bytes = t.size(dim - 1) * t.size(dim - 2) * t.size(dim - 3) * e;
-  p.stride_bytes = t.stride(dim - 4) * e;
+  const int64_t heads = t.size(dim - 3), D = t.size(dim - 1);
+  const auto is = [&](int i, int64_t stride) { return t.size(i) == 1 || t.stride(i) == stride; };
+  NEED(is(dim - 1, 1) && ((is(dim - 2, D) && is(dim - 3, D * p.page_size)) ||
+                          (is(dim - 3, D) && is(dim - 2, D * heads) && p.page_size >= 16 && p.page_size <= 256 && (p.page_size & (p.page_size - 1)) == 0)),
+       "a page must be one block of memory, [kv_heads, page_size, head_dim] or the transpose of [page_size, kv_heads, head_dim]");
+  p.page_bytes = D * p.page_size * heads * e;
+  p.stride_bytes = p.pages > 1 ? t.stride(dim - 4) * e : p.page_bytes;
   NEED(p.pages <= 1 || p.stride_bytes >= p.page_bytes, "pages must not overlap");
   p.outer = 1;
   long long stride = 0;

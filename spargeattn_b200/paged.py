@@ -4,7 +4,9 @@ The cache is plain tensors that the program owns:
 
   k_pages, v_pages  [pages, kv_heads, page_size, D] fp16 or bf16, page_size a power of two from 16 to 256; any strides with dense
                     16-byte aligned rows (a layer of one tensor [layers, 2, pages, ...], or token-major pages seen
-                    through a transpose)
+                    through a transpose). The calls that move pages take one tensor `pages` [..., pages, kv_heads, page_size, D]
+                    with all that a page number stands for (every layer's keys and values), each page one block of memory,
+                    heads or tokens first: a program that forks or compacts keeps its cache in one tensor
   page_table        [sequences, width] int32: the pages of each sequence in order, -1 behind them
   seq_lens          [sequences] int32: tokens held
   ref_counts        [pages] int32: how many sequences hold a page, 0: free

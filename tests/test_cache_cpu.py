@@ -187,3 +187,28 @@ int main() {
 ''')
     subprocess.run([gxx, "-std=c++17", "-O2", "-I", CSRC, str(src), "-o", str(tmp_path / "schedule")], check=True)
     assert subprocess.run([str(tmp_path / "schedule")]).returncode == 0
+
+
+def test_page_layouts():
+    """A page that is one block is taken in either order of its heads and tokens (and then has to be on a GPU); strides of dimensions of
+    one say nothing. Pages that interleave, or have gaps, are refused."""
+    table, lens, one = torch.zeros(2, 4, dtype=torch.int32), torch.ones(2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+
+    def calls(pool):
+        refs = torch.zeros(pool.shape[-4], dtype=torch.int32)
+        return (lambda: S.fork_sequences(pool, table, lens, refs, one, one), lambda: S.compact_pages(pool, table, refs),
+                lambda: S.copy_pages(pool, one, one))
+
+    flat = torch.zeros(8 * 16 * 64, dtype=BF)
+    for pool in (*(torch.zeros(3, 2, 8, 16, H, 64, dtype=BF).transpose(3, 4) for H in (1, 2, 16)),
+                 flat.as_strided((8, 1, 16, 64), (16 * 64, 3, 64, 1)), flat.as_strided((8, 1, 16, 64), (16 * 64, 64, 64, 1)),
+                 flat.as_strided((1, 2, 16, 64), (5, 16 * 64, 64, 1)), flat.as_strided((1, 2, 16, 64), (5, 64, 128, 1))):
+        for call in calls(pool):
+            with pytest.raises(RuntimeError, match="CUDA tensors only"):
+                call()
+    for pool in (torch.zeros(2, 16, 8, 2, 64, dtype=BF).permute(0, 2, 3, 1, 4), torch.zeros(8, 2, 32, 64, dtype=BF)[:, :, ::2],
+                 torch.zeros(8, 2, 17, 64, dtype=BF)[:, :, :16], torch.zeros(8, 16, 3, 64, dtype=BF).transpose(1, 2)[:, :2],
+                 torch.zeros(1, 1, 1, 64, dtype=BF).expand(8, 2, 16, 64), torch.zeros(8, 2, 64, 16, dtype=BF).transpose(2, 3)):
+        for call in calls(pool):
+            with pytest.raises(ValueError, match="one block"):
+                call()

@@ -779,3 +779,30 @@ def test_lse_of_rows_of_no_sequence_beside_a_given_out(chunk):
     assert (out == 7).all() and (lse == -math.inf).all()
     out, lse = S.paged_attention(q, **none, return_lse=True)
     assert (out == 0).all() and (lse == -math.inf).all()
+
+
+@pytest.mark.parametrize("H", [1, 2, 16])
+def test_bookkeeping_of_token_major_pages(H):
+    """Pages [page_size, kv_heads, D] seen through a transpose, as append_kv and paged_attention take them."""
+    ps = 32
+    pages, table, lens, refs, o = _pool(150, ps, 9, 7, H, H=H)
+    if H == 1:                                                         # what a view says about one head is not looked at
+        pages = pages.as_strided(pages.shape, (*pages.stride()[:-3], 3, *pages.stride()[-2:]))
+    else:
+        pages = pages.transpose(-2, -3).contiguous().transpose(-2, -3)
+        assert pages.stride(-3) == 64
+    g = _gen(25)
+    for step in range(3):
+        src, dst = torch.randint(0, 9, (4,), generator=g).tolist(), torch.randperm(9, generator=g)[:4].tolist()
+        assert S.fork_sequences(pages, table, lens, refs, _i32(*src), _i32(*dst)).tolist() == o.fork(src, dst)
+        new = torch.randint(0, ps, (9,), generator=g).tolist()
+        assert S.allocate_pages(table, lens, refs, _i32(*new), ps).tolist() == o.allocate(new)
+        gone = [step, 5 + step]
+        S.free_sequences(table, lens, refs, _i32(*gone))
+        o.free(gone)
+        _same(pages, table, lens, refs, o)
+        assert S.compact_pages(pages, table, refs).tolist() == [o.compact()]
+        _same(pages, table, lens, refs, o)
+    S.copy_pages(pages, _i32(140, 3), _i32(149, 148))
+    o.pages[:, 149], o.pages[:, 148] = o.pages[:, 140], o.pages[:, 3]
+    _same(pages, table, lens, refs, o)
