@@ -364,7 +364,8 @@ int sparge_paged_attention(const sparge_paged_attention_args* args, sparge_strea
  * sparge_compact_pages: live pages with numbers from the count of live pages up move into the free ones below it, in ascending
  * order both; table and counts follow. live [1]: the count. Table entries from num_pages up are left as they are.
  * sparge_copy_pages: page dst[i] becomes a copy of page src[i]. Numbers outside the pool are reported and skipped (-1 silently);
- * a pair whose destination is another pair's destination or source is reported as SPARGE_DEV_PAGE_HAZARD and not copied.
+ * a pair whose destination is another pair's destination or source is reported as SPARGE_DEV_PAGE_HAZARD and not copied (skipped
+ * pairs do not count).
  *
  * pages: `outer` times [num_pages] blocks of page_bytes (a multiple of 16) each: block p of slice o at
  * o * outer_bytes + p * page_stride_bytes. */

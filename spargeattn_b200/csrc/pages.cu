@@ -187,18 +187,22 @@ __device__ __forceinline__ void copy_tasks(const PagePool& pool, int pairs, int 
   }
 }
 
-// A block per pair and slice of the pool, so that the search for its hazards is made once for all its copies.
+// A block per pair and slice of the pool, so that the search for its hazards is made once for all its copies. Pairs that copy
+// nothing are nobody's hazard.
 __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(PagePool pool, const int32_t* src, const int32_t* dst, int n, int pages,
                                                                   int32_t* dev_status) {
   pdl_wait();
   const int i = blockIdx.x, from = src[i], to = dst[i];
-  const bool outside = from < 0 || from >= pages || to < 0 || to >= pages;
-  if (outside) {
+  const auto inside = [=](int page) { return page >= 0 && page < pages; };
+  if (!inside(from) || !inside(to)) {
     if (from != -1 && to != -1 && threadIdx.x == 0) report_page(dev_status, SPARGE_DEV_BAD_PAGE);
     return;
   }
   int clash = 0;
-  for (int j = threadIdx.x; j < n; j += kCopyThreads) clash |= (j != i && dst[j] == to) || (src[j] == to && dst[j] != to);
+  for (int j = threadIdx.x; j < n; j += kCopyThreads) {
+    const int a = src[j], b = dst[j];
+    clash |= (j != i && b == to && inside(a)) || (a == to && b != to && inside(b));
+  }
   if (__syncthreads_or(clash)) {
     if (threadIdx.x == 0) report_page(dev_status, SPARGE_DEV_PAGE_HAZARD);
     return;

@@ -100,6 +100,7 @@ def compact_pages(pages, page_table, ref_counts):
 @_skip_frame
 def copy_pages(pages, src, dst):
     """Page dst[i] becomes a copy of page src[i] in every layer that `pages` holds; pairs with -1 are skipped. A pair whose
-    destination is another pair's destination or source has no defined order: it is not copied, and reported."""
+    destination is the destination or source of another one that is not skipped has no defined order: it is not copied, and
+    reported."""
     _status(pages)
     return _binding.copy_pages(pages, src, dst)

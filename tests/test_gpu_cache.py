@@ -806,3 +806,16 @@ def test_bookkeeping_of_token_major_pages(H):
     S.copy_pages(pages, _i32(140, 3), _i32(149, 148))
     o.pages[:, 149], o.pages[:, 148] = o.pages[:, 140], o.pages[:, 3]
     _same(pages, table, lens, refs, o)
+
+
+def test_skipped_copies_stand_in_no_ones_way():
+    """A pair that is skipped, for a -1 or a page that the pool does not have, takes no part in the search for hazards."""
+    dev = torch.randn(2, 9, 1, 16, 8, generator=_gen(26)).cuda()
+    want = dev.clone()
+    # 0 -> 3 beside pairs that name page 3, or page 0, and copy nothing
+    S.copy_pages(dev, _i32(0, -1, 3, -1, 5), _i32(3, 3, -1, 0, 6))
+    want[:, 3], want[:, 6] = want[:, 0], want[:, 5]
+    assert _status() == 0 and torch.equal(dev, want)
+    S.copy_pages(dev, _i32(1, 9, 4, -5), _i32(4, 4, 2 ** 30, 1))
+    want[:, 4] = want[:, 1]
+    assert _status() == 4 and torch.equal(dev, want)
