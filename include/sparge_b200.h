@@ -360,7 +360,7 @@ int sparge_paged_attention(const sparge_paged_attention_args* args, sparge_strea
  * sparge_fork_sequences: sequence dst[i] becomes a copy of src[i] for all i at once (every source is read before any
  * destination changes). Full pages are shared; a last page that is not full is copied to a fresh page. What the
  * destinations held before is released, after the fresh pages were taken. served [n]: 0 where there was no page left, or
- * where a later pair has the same destination; such a destination stays as it was. src[i] == dst[i] does nothing.
+ * where a later pair that is not skipped has the same destination; such a destination stays as it was. src[i] == dst[i] does nothing.
  * sparge_compact_pages: live pages with numbers from the count of live pages up move into the free ones below it, in ascending
  * order both; table and counts follow. live [1]: the count. Table entries from num_pages up are left as they are.
  * sparge_copy_pages: page dst[i] becomes a copy of page src[i]. Numbers outside the pool are reported and skipped (-1 silently);

@@ -100,7 +100,9 @@ class Pool:
         served, rows = [], {}
         free = [p for p, r in enumerate(self.refs) if r == 0]
         for i, (s, d) in enumerate(zip(src, dst)):
-            if not (0 <= s < len(self.table) and 0 <= d < len(self.table)) or d in dst[i + 1:]:
+            there = lambda n: 0 <= n < len(self.table)  # noqa: E731
+            # a later pair with the same destination has it, unless that one is skipped
+            if not (there(s) and there(d)) or any(y == d and there(x) for x, y in zip(src[i + 1:], dst[i + 1:])):
                 served.append(False)
                 continue
             served.append(True)

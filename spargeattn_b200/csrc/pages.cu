@@ -220,6 +220,11 @@ struct ForkPlan {
   int32_t *state, *len, *at, *from, *to, *rows, *list;   // [n] each, rows [n][width], list [pages]
 };
 
+// Whether pair j (j > i) takes pair i's destination d from it: the later one has it, unless it is skipped.
+__device__ __forceinline__ bool takes(const PageTable& t, const int32_t* src, const int32_t* dst, int j, int d) {
+  return dst[j] == d && src[j] >= 0 && src[j] < t.sequences;
+}
+
 // Pair i by `threads` threads, of which this is number `tid`; later: whether a pair behind it has its destination.
 __device__ __forceinline__ void gather_pair(const PageTable& t, int i, int s, int d, bool later, const ForkPlan& f, int tid, int threads, int32_t* dev_status) {
   const bool inside = s >= 0 && s < t.sequences && d >= 0 && d < t.sequences;
@@ -244,7 +249,7 @@ __global__ void __launch_bounds__(256) fork_gather_kernel(PageTable t, const int
   pdl_trigger();
   const int i = blockIdx.x, d = dst[i];
   int later = 0;
-  for (int j = i + 1 + threadIdx.x; j < n; j += 256) later |= dst[j] == d;
+  for (int j = i + 1 + threadIdx.x; j < n; j += 256) later |= takes(t, src, dst, j, d);
   gather_pair(t, i, src[i], d, __syncthreads_or(later) != 0, f, threadIdx.x, 256, dev_status);
 }
 
@@ -261,7 +266,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(PageTable t, co
     for (int i = threadIdx.x >> 5; i < n; i += kPlanThreads / 32) {
       const int d = dst[i];
       int later = 0;
-      for (int j = i + 1 + lane; j < n; j += 32) later |= dst[j] == d;
+      for (int j = i + 1 + lane; j < n; j += 32) later |= takes(t, src, dst, j, d);
       gather_pair(t, i, src[i], d, __any_sync(0xffffffffu, later), f, lane, 32, dev_status);
     }
     __syncthreads();

@@ -84,7 +84,8 @@ def fork_sequences(pages, page_table, seq_lens, ref_counts, src, dst):
     """Sequence dst[i] becomes a copy of sequence src[i], for all i at once (a permutation of beams is fine). Full pages are
     shared; a last page that is not full is copied to a fresh one, in every layer that `pages` [..., pages, kv_heads, page_size, D]
     holds, so that both may go on writing. What the destinations held is released afterwards. Returns served [len(src)] bool: False
-    where no page was left, or where a later pair has the same destination; such a destination stays as it was."""
+    where no page was left (the destination stays as it was), where the pair is skipped (-1), or where a later pair that is not
+    skipped has the same destination."""
     _status(pages)
     return _binding.fork_sequences(pages, page_table, seq_lens, ref_counts, src, dst)
 

@@ -819,3 +819,22 @@ def test_skipped_copies_stand_in_no_ones_way():
     S.copy_pages(dev, _i32(1, 9, 4, -5), _i32(4, 4, 2 ** 30, 1))
     want[:, 4] = want[:, 1]
     assert _status() == 4 and torch.equal(dev, want)
+
+
+# few pairs, planned in one kernel, and many
+@pytest.mark.parametrize("n", [3, 600])
+def test_skipped_forks_stand_in_no_ones_way(n):
+    """A pair that is skipped, for a -1 or a sequence that there is not, does not take its destination from another one."""
+    sequences, ps = 2 * n, 16
+    pages, table, lens, refs, o = _pool(8 * sequences, ps, sequences, 6, n, (1,), 1)
+    g = _gen(27)
+    src, dst = torch.randint(0, n, (n,), generator=g).tolist(), list(range(n, 2 * n))
+    skipped = [-1] * n
+    assert S.fork_sequences(pages, table, lens, refs, _i32(*src, *skipped), _i32(*dst, *dst)).tolist() == [True] * n + [False] * n
+    assert _status() == 0
+    assert o.fork(src + skipped, dst + dst) == [True] * n + [False] * n
+    _same(pages, table, lens, refs, o)
+    skipped = [sequences] * n
+    assert S.fork_sequences(pages, table, lens, refs, _i32(*src, *skipped), _i32(*dst, *dst)).tolist() == o.fork(src + skipped, dst + dst)
+    assert _status() == 4
+    _same(pages, table, lens, refs, o)
