@@ -306,8 +306,9 @@ typedef struct {
  * sequence on the way (pairs, interleaved, magnitude as in sparge_rotary), and q [tokens, q_heads, D], if given, to q_out.
  * Strides {token, head}. Rows of no sequence are not written to pages and give zeros in q_out. A token whose position
  * has no page (table entry outside the pool, position below 0 or outside the table) is left out of the pages and reported as
- * SPARGE_DEV_BAD_PAGE. Two tokens never share a place unless two sequences
- * share the page that they write to, which is the caller's mistake. */
+ * SPARGE_DEV_BAD_PAGE. Rows of a sequence with served 0 are treated as rows of no sequence: its length does not include
+ * them, so that their places hold keys of its own, and of forks that share the page. Else two tokens never share a place
+ * unless two sequences share the page that they write to, which is the caller's mistake. */
 typedef struct {
   sparge_cache cache;
   const void *k, *v, *q;
@@ -318,6 +319,7 @@ typedef struct {
   int pairs, interleaved;
   float magnitude;
   int32_t* dev_status;
+  const unsigned char* served; /* [sequences], of sparge_allocate_pages, or NULL */
 } sparge_append_args;
 int sparge_append_kv(const sparge_append_args* args, sparge_stream_t stream);
 

@@ -309,9 +309,9 @@ void cache_on_gpu(const CacheTensors& t, c10::Device dev) {
   if (t.cu) on_gpu(*t.cu, dev, "cu_seqlens");
 }
 
-// (k, v, k_pages, v_pages, page_table, seq_lens, cu_seqlens, q, frequencies, interleaved, magnitude) -> q' or None
+// (k, v, k_pages, v_pages, page_table, seq_lens, cu_seqlens, q, frequencies, interleaved, magnitude, served or None) -> q' or None
 PyObject* append_impl(PyObject* const* args, Py_ssize_t nargs) {
-  arguments(nargs, 11, "append_kv");
+  arguments(nargs, 12, "append_kv");
   const Tensor &k = tensor(args[0], "k"), &v = tensor(args[1], "v");
   NEED(k.dim() == 3 && v.dim() == 3 && k.sizes() == v.sizes(), "k and v must be [tokens, kv_heads, head_dim] of one shape");
   NEED(k.scalar_type() == v.scalar_type(), "k and v must have the same type");
@@ -336,8 +336,15 @@ PyObject* append_impl(PyObject* const* args, Py_ssize_t nargs) {
   const double magnitude = number(args[10], "magnitude");
   NEED(std::isfinite(magnitude), "magnitude must be finite");
   a.magnitude = (float)magnitude;
+  const Tensor* served = args[11] == Py_None ? nullptr : &tensor(args[11], "served");
+  if (served) {
+    NEED(served->scalar_type() == at::kBool && served->dim() == 1 && served->is_contiguous(), "served must be a contiguous bool vector");
+    NEED(served->numel() == a.cache.sequences, "served must have an element for each of the ", a.cache.sequences, " sequences, has ", served->numel());
+    a.served = (const unsigned char*)served->data_ptr();
+  }
   const c10::Device dev = k.device();
   on_gpu(k, dev, "k"), on_gpu(v, dev, "v");
+  if (served) on_gpu(*served, dev, "served");
   cache_on_gpu(t, dev);
   if (q) on_gpu(*q, dev, "q");
   if (freq) on_gpu(*freq, dev, "frequencies");

@@ -46,6 +46,7 @@ struct RotParams {
   int tokens_per_block, tok_shift;   // a power of two
   // append
   const int32_t *table, *seq_lens, *cu;
+  const unsigned char* served;
   long long table_stride;
   int sequences, width, num_pages, page_size;
   int32_t* dev_status;
@@ -186,7 +187,7 @@ __device__ __forceinline__ RotShare rot_share(const RotParams& p, const RotSlot&
 template <typename T, int V, bool VEC, bool INTER, bool PAGED, bool ROT>
 __global__ void __launch_bounds__(kRotThreads, (RotShape<INTER, ROT>::kBlocks)) rotary_kernel(const __grid_constant__ RotParams p) {
   extern __shared__ float2 s_cs[];                  // [tokens_per_block][pairs]
-  __shared__ int s_page[kRotTokens], s_row[kRotTokens], s_pos[kRotTokens];   // paged: -1 no page; row -1 behind the last sequence
+  __shared__ int s_page[kRotTokens], s_row[kRotTokens], s_pos[kRotTokens];   // paged: -1 no page; row -1 of no sequence, or of one not served
   __shared__ int s_seq;
   const int tid = threadIdx.x, TOK = p.tokens_per_block;
   const long long tokens = (long long)p.B * p.N, t0 = (long long)blockIdx.x * TOK;
@@ -217,7 +218,7 @@ __global__ void __launch_bounds__(kRotThreads, (RotShape<INTER, ROT>::kBlocks)) 
         } else {
           seq = (int)t;
         }
-        if (seq < p.sequences) {
+        if (seq < p.sequences && (!p.served || p.served[seq])) {
           const long long at = (long long)p.seq_lens[seq] - (end - t);
           row = 0;
           if (at >= 0 && at < (long long)p.width * p.page_size) {
@@ -407,7 +408,7 @@ extern "C" int sparge_append_kv(const sparge_append_args* a, sparge_stream_t str
   paged(a->k, a->k_st, c.k_pages, c.k_st, a->frequencies != nullptr);
   paged(a->v, a->v_st, c.v_pages, c.v_st, false);
   p.B = 1, p.N = c.tokens, p.D = c.D, p.pairs = a->frequencies ? a->pairs : 0, p.axes = 1, p.freq = a->frequencies, p.magnitude = a->magnitude;
-  p.table = c.page_table, p.seq_lens = c.seq_lens, p.cu = c.cu_seqlens, p.table_stride = c.table_stride;
+  p.table = c.page_table, p.seq_lens = c.seq_lens, p.cu = c.cu_seqlens, p.served = a->served, p.table_stride = c.table_stride;
   p.sequences = c.sequences, p.width = c.table_width, p.num_pages = c.num_pages, p.page_size = c.page_size, p.dev_status = a->dev_status;
   return rotary_dispatch<true>(p, a->interleaved != 0, c.dtype, (cudaStream_t)stream);
 }

@@ -11,10 +11,10 @@ The cache is plain tensors that the program owns:
   seq_lens          [sequences] int32: tokens held
   ref_counts        [pages] int32: how many sequences hold a page, 0: free
 
-A step: `allocate_pages` grows the sequences (seq_lens then include the new tokens), and each layer calls `append_kv` and
-`paged_attention`. New tokens are packed, [tokens, heads, D]: sequence i has the rows cu_seqlens[i] to cu_seqlens[i + 1], its last
-tokens; without cu_seqlens every sequence has one. No function synchronises or copies to the host, and lengths, tables and
-cu_seqlens are read when the kernels run, so a captured step follows them from replay to replay.
+A step: `allocate_pages` grows the sequences (seq_lens then include the new tokens) and says which it served, and each layer calls
+`append_kv`, with that, and `paged_attention`. New tokens are packed, [tokens, heads, D]: sequence i has the rows cu_seqlens[i] to
+cu_seqlens[i + 1], its last tokens; without cu_seqlens every sequence has one. No function synchronises or copies to the host,
+and lengths, tables and cu_seqlens are read when the kernels run, so a captured step follows them from replay to replay.
 
 Arguments that do not fit are ValueError, CPU tensors RuntimeError. What only the device can see (a page number outside the
 pool, a length outside the table) is skipped without touching other memory and reported through `ops.check_device_status()`.
@@ -36,15 +36,21 @@ def _status(t):
 
 
 @_skip_frame
-def append_kv(k, v, k_pages, v_pages, page_table, seq_lens, cu_seqlens=None, q=None, frequencies=None, interleaved=False, magnitude=1.0):
+def append_kv(k, v, k_pages, v_pages, page_table, seq_lens, cu_seqlens=None, q=None, frequencies=None, interleaved=False,
+              magnitude=1.0, served=None):
     """Writes the new tokens' k and v [tokens, kv_heads, D] to their pages. seq_lens include them.
 
     With `frequencies` (see `apply_rotary`) k is turned by its position in the sequence on the way, and q [tokens, heads, D], if
     given, is turned too and returned (rows of no sequence: zeros): one pass over the layer's projections. Else returns
-    None. A token whose position has no page is left out and reported. Sequences that share the page they write to (which
-    `fork_sequences` never leaves behind) are the caller's mistake."""
+    None. A token whose position has no page is left out and reported.
+
+    `served` [sequences] bool, as `allocate_pages` returned it, leaves out the tokens of sequences that it did not serve (their q
+    becomes zeros, and what attention makes of that means nothing). Where the pool or a row of the table may run out it is needed:
+    such a sequence kept its length, so its tokens would fall on its last positions, over keys that it holds, and that
+    its forks may share. Sequences that share the page they write to otherwise (a served sequence never does, after
+    `fork_sequences` and `allocate_pages`) are the caller's mistake."""
     _status(k)
-    return _binding.append_kv(k, v, k_pages, v_pages, page_table, seq_lens, cu_seqlens, q, frequencies, interleaved, magnitude)
+    return _binding.append_kv(k, v, k_pages, v_pages, page_table, seq_lens, cu_seqlens, q, frequencies, interleaved, magnitude, served)
 
 
 @_skip_frame

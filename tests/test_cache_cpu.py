@@ -212,3 +212,13 @@ def test_page_layouts():
         for call in calls(pool):
             with pytest.raises(ValueError, match="one block"):
                 call()
+
+
+@pytest.mark.parametrize("served,text", [(torch.ones(2, dtype=torch.int32), "bool"), (torch.ones(3, dtype=torch.bool), "sequences"),
+                                         (torch.ones(2, 1, dtype=torch.bool), "bool"), (torch.ones(4, dtype=torch.bool)[::2], "bool")])
+def test_append_refuses_served(served, text):
+    k = torch.zeros(2, 2, 64, dtype=BF)
+    with pytest.raises(ValueError, match=text):
+        S.append_kv(k, k, **_cache(), served=served)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        S.append_kv(k, k, **_cache(), served=torch.ones(2, dtype=torch.bool))

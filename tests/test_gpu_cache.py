@@ -838,3 +838,54 @@ def test_skipped_forks_stand_in_no_ones_way(n):
     assert S.fork_sequences(pages, table, lens, refs, _i32(*src, *skipped), _i32(*dst, *dst)).tolist() == o.fork(src + skipped, dst + dst)
     assert _status() == 4
     _same(pages, table, lens, refs, o)
+
+
+@pytest.mark.parametrize("chunks", [None, [1, 1, 1, 1], [3, 2, 20, 0]])
+@pytest.mark.parametrize("rotated", [False, True])
+def test_append_to_sequences_that_were_not_served(chunks, rotated):
+    """A sequence that the pool had no room for keeps what it holds, and so does one that shares its pages; a captured step too."""
+    ps, H, D = 16, 2, 64
+    ragged = chunks is not None
+    kv = torch.randn(2, 5, H, ps, D, generator=_gen(28)).to(BF).cuda()
+    table, lens, refs = torch.full((4, 3), -1, dtype=torch.int32).cuda(), _i32(0, 0, 0, 0), torch.zeros(5, dtype=torch.int32).cuda()
+    assert S.allocate_pages(table, lens, refs, _i32(2 * ps, 0, 5, ps), ps).all()                       # 4 of 5 pages
+    assert S.fork_sequences(kv, table, lens, refs, _i32(0), _i32(1)).all()                             # ends with a page: shared
+    new = _i32(*(chunks or [1] * 4))
+    cut = _i32(*_cu(chunks)) if ragged else None
+    T = sum(chunks) if ragged else 4
+    g = _gen(29)
+    q, k, v = (torch.randn(T, h, D, generator=g).to(BF).cuda() for h in (4, H, H))
+    freq = S.rotary_frequencies(D)[0] if rotated else None
+    ops.device_status_word(q.device)
+    table0, lens0, refs0, kv0 = table.clone(), lens.clone(), refs.clone(), kv.clone()
+
+    def step():
+        served = S.allocate_pages(table, lens, refs, new, ps)
+        return served, S.append_kv(k, v, kv[0], kv[1], table, lens, cut, q=q if rotated else None, frequencies=freq, served=served)
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    results = []
+    for run in (lambda: captured if graph.replay() is None else None, step):
+        for a, b in ((table, table0), (lens, lens0), (refs, refs0), (kv, kv0)):
+            a.copy_(b)
+        served, turned = run()
+        results.append((served.clone(), None if turned is None else turned.clone(), kv.clone()))
+        got, held = served.tolist(), lens.tolist()
+        assert got == ([True, False, True, False] if chunks is None or chunks[2] == 1 else [True, False, False, True])
+        want = kv0.cpu()
+        for i, (t0, t1) in enumerate(zip(_cu(chunks or [1] * 4)[:-1], _cu(chunks or [1] * 4)[1:])):
+            for t in range(t0, t1):
+                p = held[i] - (t1 - t)
+                if not got[i]:
+                    assert not rotated or (turned[t] == 0).all()
+                    continue
+                page = table[i, p // ps].item()
+                want[1, page, :, p % ps] = v[t].cpu()
+                want[0, page, :, p % ps] = kv[0, page, :, p % ps].cpu() if rotated else k[t].cpu()
+                if rotated:
+                    _check_rotary(kv[0, page, :, p % ps], k[t], p * freq.cpu(), False)
+                    _check_rotary(turned[t], q[t], p * freq.cpu(), False)
+        assert torch.equal(kv.cpu(), want)                             # nothing else was written
+    assert torch.equal(results[0][2], results[1][2]) and torch.equal(results[0][0], results[1][0])
