@@ -7,6 +7,7 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/Exceptions.h>
@@ -229,11 +230,27 @@ struct RotaryTwo : torch::autograd::Function<RotaryTwo> {
   }
 };
 
+std::pair<Tensor, Tensor> rotary_dual(const Tensor& q, const Tensor* k, const Tensor& pos, const Tensor& freq, const RotaryHow& how);
+
 std::pair<Tensor, Tensor> rotary_grad(const Tensor& q, const Tensor* k, const Tensor& pos, const Tensor& freq, const RotaryHow& how) {
+  if ((q._fw_grad(0).defined() || (k && k->_fw_grad(0).defined())) && c10::AutogradState::get_tls_state().get_fw_grad_mode())
+    return rotary_dual(q, k, pos, freq, how);
   if (!at::GradMode::is_enabled() || !(q.requires_grad() || (k && k->requires_grad()))) return rotary_run(q, k, pos, freq, how);
   if (!k) return {RotaryOne::apply(q, pos, freq, how), Tensor()};
   const auto r = RotaryTwo::apply(q, *k, pos, freq, how);
   return {r[0], r[1]};
+}
+
+// Forward mode: values and tangents turn alike, each by a call of its own, differentiable as ever.
+std::pair<Tensor, Tensor> rotary_dual(const Tensor& q, const Tensor* k, const Tensor& pos, const Tensor& freq, const RotaryHow& how) {
+  const Tensor tq = q._fw_grad(0), tk = k ? k->_fw_grad(0) : Tensor(), vk = k ? k->_fw_primal(0) : Tensor();
+  auto r = rotary_grad(q._fw_primal(0), k ? &vk : nullptr, pos, freq, how);
+  std::pair<Tensor, Tensor> t;
+  if (tq.defined()) t = rotary_grad(tq, tk.defined() ? &tk : nullptr, pos, freq, how);
+  else t.second = rotary_grad(tk, nullptr, pos, freq, how).first;
+  if (t.first.defined()) r.first._set_fw_grad(t.first, 0, false);
+  if (t.second.defined()) r.second._set_fw_grad(t.second, 0, false);
+  return r;
 }
 
 // (q, k or None, positions, frequencies, interleaved, sections or None, magnitude, layout) -> q' or (q', k')

@@ -70,7 +70,8 @@ def apply_rotary(q, k, positions, frequencies, interleaved=False, sections=None,
     channels behind them are copied. `interleaved`: pairs are neighbours (2 i, 2 i + 1), else (i, i + pairs). `positions`: int32 or
     int64 [N] or [B, N]. With `sections` (pairs per axis, in order) positions have an axis of that length in front, and a
     pair turns by the position on its axis: frame, row and column of a video. Angles are formed in 64 bits, so far
-    positions lose nothing. Differentiable in q and k; the gradient is turned back by the same kernel.
+    positions lose nothing. Differentiable in q and k; the gradient is turned back by the same kernel, and
+    tangents of forward mode are turned like their values.
 
     Work is queued on the current stream. Shapes, types and ranges that do not fit are ValueError, CPU tensors RuntimeError."""
     return _binding.rotary(q, k, positions, frequencies, interleaved, sections, magnitude, tensor_layout)

@@ -889,3 +889,32 @@ def test_append_to_sequences_that_were_not_served(chunks, rotated):
                     _check_rotary(turned[t], q[t], p * freq.cpu(), False)
         assert torch.equal(kv.cpu(), want)                             # nothing else was written
     assert torch.equal(results[0][2], results[1][2]) and torch.equal(results[0][0], results[1][0])
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_forward_mode(interleaved):
+    """The tangent of a dual tensor is turned like its value, with and without a backward graph beside it."""
+    import torch.autograd.forward_ad as fw
+    g = _gen(30)
+    freq = S.rotary_frequencies(48)[0]
+    pos = torch.tensor([5, 90_000, 3], dtype=torch.int32)
+    phase = pos.double()[:, None] * freq.cpu()
+    q, k, tq, tk, w = (torch.randn(2, h, 3, 64, generator=g) for h in (3, 1, 3, 1, 3))
+    turn = lambda a, b: S.apply_rotary(a, b, pos.cuda(), freq, interleaved, magnitude=0.75)  # noqa: E731
+    with fw.dual_level():
+        dual = fw.make_dual(q.cuda(), tq.cuda())
+        for a in (turn(dual, None), turn(dual, k.cuda())[0], turn(k.cuda(), dual)[1]):
+            value, tangent = fw.unpack_dual(a)
+            _check_rotary(value, q, phase, interleaved, 0.75)
+            _check_rotary(tangent, tq, phase, interleaved, 0.75)
+        assert fw.unpack_dual(turn(dual, k.cuda())[1]).tangent is None
+        # both of them, in half the bits, token-major
+        dq, dk = (fw.make_dual(x.to(BF).cuda().transpose(1, 2), t.to(BF).cuda().transpose(1, 2)) for x, t in ((q, tq), (k, tk)))
+        for a, x in zip(S.apply_rotary(dq, dk, pos.cuda(), freq, interleaved, tensor_layout="NHD"), (tq, tk)):
+            _check_rotary(fw.unpack_dual(a).tangent.transpose(1, 2), x.to(BF), phase, interleaved)
+        # beside a backward graph: the value's gradient, and the tangent's
+        leaf, along = q.cuda().requires_grad_(), tq.cuda().requires_grad_()
+        value, tangent = fw.unpack_dual(turn(fw.make_dual(leaf, along), k.cuda())[0])
+        _check_rotary(tangent.detach(), tq, phase, interleaved, 0.75)
+        _check_rotary(torch.autograd.grad(value, leaf, w.cuda(), retain_graph=True)[0], w, -phase, interleaved, 0.75)
+        _check_rotary(torch.autograd.grad(tangent, along, w.cuda())[0], w, -phase, interleaved, 0.75)
