@@ -372,7 +372,10 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       const int r = x * 128 + local, seq_row = w.row + r, tok = seq_row / p.group;
       const bool mine = r < w.rows, idle = x * 128 + (warp & 3) * 32 >= w.rows;   // no row of this warp is in the tile
       const int limit = mine ? min(w.length, w.visible0 + (p.causal ? tok + 1 : 0)) : 0;
-      float m = -INFINITY, l = 0.f;
+      // A score s weighs 2^((s - sub) c + off): off is -m c as it is rounded, the same for every key (what it is off by goes out in the
+      // division), so that a weight takes one instruction and one rounding. Where off could be off by whole powers of two m is
+      // subtracted first (sub; else 0).
+      float m = -INFINITY, l = 0.f, sub = 0.f, off = 0.f;
       const int here = w.units, key0 = w.key;
       for (int j = 0; j < here; j++) {
         mbar_wait_or_flag(&bar_s[x], phase, &s_fail, SPARGE_DEV_TIMEOUT_SOFTMAX);
@@ -394,8 +397,12 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
           }
           const float mx = fmaxf(row_max(s), m);
           if (__any_sync(0xffffffffu, (mx - m) * c > kRescaleFrom)) {   // (from minus infinity: always; both: NaN, never)
-            const float alpha = mx == -INFINITY ? 1.f : ex2_approx((m - mx) * c);
-            m = mx;
+            const float shift = mx == -INFINITY ? 0.f : -mx * c;
+            const bool far = fabsf(shift) > 1048576.f;
+            const float sub_to = far ? mx : 0.f, off_to = far ? 0.f : shift;
+            // what the earlier weights have to be multiplied by, from the very numbers that they were formed with
+            const float alpha = m == -INFINITY ? 0.f : ex2_approx(fmaf(sub - sub_to, c, off_to - off));
+            m = mx, sub = sub_to, off = off_to;
             l *= alpha;
             if (j > 0) {   // the products up to the step before are in O: S of this step came behind them
 #pragma unroll
@@ -409,13 +416,9 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
               }
             }
           }
-          // s c - m c in one rounding: what m c is off by is the same for the whole row, and goes out in the division. Where it
-          // could be off by whole powers of two the difference is taken first.
-          float off = m == -INFINITY ? 0.f : -m * c;
-          if (__any_sync(0xffffffffu, fabsf(off) > 1048576.f)) {
+          if (__any_sync(0xffffffffu, sub != 0.f)) {
 #pragma unroll
-            for (int k = 0; k < kBlockKeys; k++) s[k] -= m == -INFINITY ? 0.f : m;
-            off = 0.f;
+            for (int k = 0; k < kBlockKeys; k++) s[k] -= sub;
           }
           const float2 c2 = make_float2(c, c), off2 = make_float2(off, off);
           float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);

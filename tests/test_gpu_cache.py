@@ -918,3 +918,35 @@ def test_rotary_forward_mode(interleaved):
         _check_rotary(tangent.detach(), tq, phase, interleaved, 0.75)
         _check_rotary(torch.autograd.grad(value, leaf, w.cuda(), retain_graph=True)[0], w, -phase, interleaved, 0.75)
         _check_rotary(torch.autograd.grad(tangent, along, w.cuda())[0], w, -phase, interleaved, 0.75)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("neighbour", [False, True])
+def test_maximum_that_moves_far_from_zero(dtype, neighbour):
+    """Scores near 2^20 in base 2: what the keys before a larger one weigh is what they weigh beside it, to the bits of their difference.
+
+    The products are whole numbers, so the scores are exact. 2 432 equal keys, then one that is larger by one unit of 11.3 in base 2: the
+    old ones weigh 2 432 x 2^-11.3 of it. With `neighbour` another row of the same warp goes beyond 2^20 half way.
+    Errors: a probability's rounding to the type eps / 2 of its share and the output's own; exponents of up to 12 in 32 bits, their
+    exponentials, and sums of up to 64 + 20 terms in a row: together under 1e-5 of the whole."""
+    H, D, ps, n = 148, 64, 64, 2560                                    # a tile for each multiprocessor, so that steps follow each other
+    B, scale = 64256.0, 7.84375                                        # 251 x 2^8; scale in base 2 is 11.316
+    K, V = torch.zeros(n, D), torch.zeros(n, D)
+    K[:, 0], K[n - 128:, 1], K[n - 1, 1] = B, -10.0, 1.0
+    V[: n - 128], V[n - 1] = -1.0, 1.0
+    K[n // 2:, 2] = 32768.0
+    q = torch.zeros(20, H, D)
+    q[..., :2] = 1.0
+    if neighbour:
+        q[5, :, 2] = 8.0
+    c = dict(seq_lens=_i32(n), page_table=torch.arange(n // ps, dtype=torch.int32).cuda()[None])
+    for name, x in (("k_pages", K), ("v_pages", V)):
+        c[name] = x.view(n // ps, 1, ps, D).expand(-1, H, -1, -1).contiguous().to(dtype).cuda()
+    out, lse = S.paged_attention(q.to(dtype).cuda(), **c, cu_seqlens=_i32(0, 20), max_chunk=20, is_causal=False, scale=scale, return_lse=True)
+    x = q[:, 0].double() @ K.double().T * scale
+    p = torch.softmax(x, -1)
+    want, weight = p @ V.double(), p @ V.double().abs()
+    room = torch.finfo(dtype).eps / 2 * (want.abs() + weight) * 1.01 + 1e-5 + (2.0 ** -25 * (1 + n) if dtype == HF else 0.0)
+    off = (out.cpu().double() - want[:, None]).abs() - room[:, None]
+    assert (off <= 0).all(), off.max()
+    assert ((lse.cpu().double() - torch.logsumexp(x, -1)[:, None]).abs() <= 2.0 ** -21 * x.abs().max()).all()
