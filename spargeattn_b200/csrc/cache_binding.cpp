@@ -159,7 +159,7 @@ std::pair<Tensor, Tensor> rotary_run(const Tensor& q, const Tensor* k_or_null, c
   a.positions_st[2] = pos.stride(lead + pd - 1);
   a.positions = pos.data_ptr();
   a.interleaved = how.interleaved, a.inverse = how.inverse;
-  NEED(std::isfinite(how.magnitude), "magnitude must be finite");
+  NEED(std::isfinite((float)how.magnitude), "magnitude must be finite in 32 bits");
   a.magnitude = (float)how.magnitude;
   const c10::Device dev = q.device();
   on_gpu(q, dev, "q"), on_gpu(k, dev, "k"), on_gpu(pos, dev, "positions"), on_gpu(freq, dev, "frequencies");
@@ -351,7 +351,7 @@ PyObject* append_impl(PyObject* const* args, Py_ssize_t nargs) {
     if (x) NEED(x->stride(2) == 1, "the last dimension of k, v and q must be dense");
   a.interleaved = truth(args[9]);
   const double magnitude = number(args[10], "magnitude");
-  NEED(std::isfinite(magnitude), "magnitude must be finite");
+  NEED(std::isfinite((float)magnitude), "magnitude must be finite in 32 bits");
   a.magnitude = (float)magnitude;
   const Tensor* served = args[11] == Py_None ? nullptr : &tensor(args[11], "served");
   if (served) {

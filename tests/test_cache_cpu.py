@@ -222,3 +222,12 @@ def test_append_refuses_served(served, text):
         S.append_kv(k, k, **_cache(), served=served)
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
         S.append_kv(k, k, **_cache(), served=torch.ones(2, dtype=torch.bool))
+
+
+def test_magnitudes_beyond_32_bits_are_refused():
+    """A factor that is finite in 64 bits and infinite in the kernels' 32."""
+    q, k = torch.zeros(1, 2, 5, 64, dtype=BF), torch.zeros(2, 2, 64, dtype=BF)
+    for call in (lambda: S.apply_rotary(q, None, torch.zeros(5, dtype=torch.int32), _freq(8), magnitude=1e39),
+                 lambda: S.append_kv(k, k, **_cache(), frequencies=_freq(8), magnitude=-1e39)):
+        with pytest.raises(ValueError, match="finite"):
+            call()
