@@ -371,7 +371,8 @@ int sparge_paged_attention(const sparge_paged_attention_args* args, sparge_strea
  *
  * pages: `outer` times [num_pages] blocks of page_bytes (a multiple of 16) each: block p of slice o at
  * o * outer_bytes + p * page_stride_bytes. */
-enum { SPARGE_MAX_PAIRS = 65536 }; /* of one call that forks or copies: each is compared with all others */
+enum { SPARGE_MAX_PAIRS = 65536 }; /* of one call that forks or copies: each is compared with all others. Pages of 256 bytes,
+                                      us to copy / to fork: 1 024 pairs 7 / 18, 8 192 62 / 43, 65 536 6 090 / 807 */
 size_t sparge_pages_workspace_bytes(int n, int table_width, int num_pages);
 int sparge_allocate_pages(int32_t* page_table, int32_t* seq_lens, int32_t* ref_counts, const int32_t* new_tokens,
                           unsigned char* served, void* workspace, int sequences, int table_width, long long table_stride,

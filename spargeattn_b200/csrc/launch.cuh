@@ -1,9 +1,12 @@
 // Kernel launches inside one call: the kernels of a call run back to back on one stream and each depends on the one
 // before it. A programmatic dependent launch lets the next kernel's blocks start while the last ones of the current
 // kernel drain; pdl_wait() is where a kernel first touches what the kernels before it wrote (it returns when they have
-// completed and their writes are visible), pdl_trigger() lets the next one be scheduled. The trigger stands at a kernel's
-// end: given at its start, blocks of the next kernel sat in slots that the current one still needed (a [1,24,4608,128]
-// call took 207 us, 195 without dependent launches, 188 like this). Without the launch attribute both are no-ops.
+// completed and their writes are visible), pdl_trigger() lets the next one be scheduled. In the sparse attention's path the
+// trigger stands at a kernel's end: given at its start, blocks of the next kernel sat in slots that the current one still needed
+// (a [1,24,4608,128] call took 207 us, 195 without dependent launches, 188 like this). The rotation and the bookkeeping of pages
+// give it right behind their own wait: their calls of a step are one block, or a few short ones, and what comes next starts up
+// under them. Either is right, since every kernel waits before it touches what another one writes. Without the launch attribute
+// both are no-ops.
 // No block leaves a kernel in front of pdl_wait() by a return: if all of them did, the kernel would end before the one it
 // depends on, and what follows on the stream (the next user of the workspace) waits for this one only.
 // A kernel with a pdl_wait() takes no `const T* __restrict__`: that promises data which nothing writes while the kernel runs,

@@ -19,8 +19,9 @@ namespace sparge {
 
 constexpr int kBlockKeys = 128;
 
-// sum over i in [0, n) of floor((a + b i) / m), for m > 0: the number of lattice points under a line, counted by exchanging the
-// axes as in Euclid's algorithm.
+// sum over i in [0, n) of floor((a + b i) / m), for m > 0: the floor sum of an arithmetic progression, which counts the lattice points
+// under a line. By its reciprocity law (Graham, Knuth, Patashnik, Concrete Mathematics, 3.5): whole parts of the slope and of the
+// start are taken out, then the axes change places, as in Euclid's algorithm.
 SPARGE_SCHED unsigned long long floor_sum(unsigned long long n, unsigned long long a, unsigned long long b, unsigned long long m) {
   unsigned long long sum = 0;
   while (n > 0) {

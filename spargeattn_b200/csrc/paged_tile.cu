@@ -14,10 +14,13 @@
 // heads and sequences, and a tile's queries are fetched while the last product of the tile before it is under way.
 //
 // The products of a step of 128 keys take 2 048 cycles for the two tiles at D = 128 and the exponentials as many (16 a cycle on
-// an SM), so both would have to run all the time; measured: 3 300 cycles a step, tensor cores 63 % and the exponential unit 65 %
+// an SM), so both would have to run all the time; measured: 3 330 cycles a step, tensor cores 62 % and the exponential unit 65 %
 // busy, 1.10 PFLOP/s for 4 096 tokens over 20 477 keys, 32 heads to 8 (0.66 of the measured bf16 rate). What bounds it is the chain
-// of one tile: S 385 cycles after its products are asked for, 100 to read it, 260 for the maximum, the exponentials, then P V and
-// the next Q K^T, which has to wait because P lies over S. At D = 64 the products are half of that and the chain is the same.
+// of one tile (stamps of a warp, medians): 650 cycles of waiting for S, 130 to read it, 430 for the maximum, 1 780 for the
+// exponentials and the hand-over of P, then P V and the next Q K^T, which has to wait because P lies over S. At D = 64 the products are
+// half of that, and a step inside a tile takes the same 3 400 cycles (510 of them waiting for S); over a launch of ragged chunks
+// (nine of 172 to 700 tokens over up to 5 003 keys, 16 heads) it is 4 410: a share has two or three tiles, and at the end of each the
+// products wait until the next one's queries, which are fetched after the last exponentials, have arrived.
 // The running maximum moves only when a row's maximum grows by more than 2^8 (probabilities up to 256 round as exactly as ones up
 // to 1), so that the output is hardly ever rescaled. The rounding of the probabilities to the 16-bit type is the products': it
 // costs 2^-9 (2^-12) of each one's share, as much as the rounding of the output itself.

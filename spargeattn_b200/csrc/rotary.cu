@@ -17,10 +17,11 @@ constexpr int kRotThreads = 256;
 constexpr int kRotTokens = 8;      // most tokens of a block: a power of two
 
 // What keeps HBM busy is blocks on an SM, and heads loaded together; both take registers. Forward and backward pass of
-// [1,12,32760,128] queries and keys, neighbouring pairs: six blocks of two heads 144 us, five 151, seven 160 (they spill), four of
-// four heads 153, eight of one 164. A unit of two halves needs more: partial rotation of [4097, 16 + 4, 128] with four blocks 10.0
-// us, five 14.1, six 25.7. Without a rotation there is nothing else to hold: four heads (17.0 us for 9 450 tokens' keys and values,
-// two 19.1). Tokens of a block: eight 144 us, four 176, sixteen 150.
+// [1,12,32760,128] bf16 queries and keys, neighbouring pairs: six blocks of two heads 144 us (20 bytes of a thread spilled), five 151,
+// seven 160, four of four heads 153, eight of one 164. A unit of two halves needs more: partial rotation of fp16 [4097, 16 + 4, 128] with
+// four blocks 10.0 us (11.0 in later runs), five 14.1, six 25.7. Without a rotation there is nothing else to hold: four heads (17.0 us for
+// 9 450 tokens' keys and values, two 19.1). Tokens of a block: eight 144 us, four 176, sixteen 150. fp32 takes the same shapes and spills
+// more (76 bytes of neighbouring pairs, 114 of half-apart ones); it was not timed apart.
 template <bool INTER, bool ROT>
 struct RotShape {
   static constexpr int kAhead = ROT ? 2 : 4, kBlocks = ROT && INTER ? 6 : 4;
