@@ -18,11 +18,12 @@ and lengths, tables and cu_seqlens are read when the kernels run, so a captured 
 
 Lengths grow by `allocate_pages` and go back to 0 by `free_sequences`. A program that lowers one itself (drafted tokens that were
 rejected) also sets the entries of the pages behind it to -1 and takes one off their counts: `allocate_pages` writes over
-what stands there, and a page whose entry is gone keeps its count.
+what stands there, and a page whose entry is gone keeps its count. It does not go back into a page that a fork shares: the next
+token would be written for both.
 
 Arguments that do not fit are ValueError, CPU tensors RuntimeError. What only the device can see (a page number outside the
-pool, a length outside the table) is skipped without touching other memory and reported through `ops.check_device_status()`; the first report stays
-until `ops.device_status_word(device).zero_()`.
+pool, a length outside the table) is skipped without touching other memory and reported through `ops.check_device_status()`; the
+first report stays until `ops.device_status_word(device).zero_()`.
 Nothing here has a gradient. The first call on a device should precede graph capture: it sets up the word that reports go to.
 """
 import torch
